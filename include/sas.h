@@ -29,6 +29,10 @@
  *       layout of the reference's generators golden.py:315-360 (the inverse of
  *       unpack_paged_kv, golden.py:247-268).  The reference has no device
  *       writer: its tests build the caches on the host.
+ *   sas_norm_rope / sas_kv_append_norm_rope
+ *       the norm and rotation of query heads and of key rows on their way into
+ *       a paged cache, the step before the path; the reference takes both
+ *       already transformed (api.py:129-153).
  *   sas_error_string / sas_version
  *       error reporting in place of the reference's Python asserts
  *       (api.py:187-191, 279-282).
@@ -63,7 +67,7 @@ enum {
 /* ---- layouts / modes / dtypes (values of the reference's string enums) ---- */
 enum { SAS_LAYOUT_BSND = 0, SAS_LAYOUT_TND = 1, SAS_LAYOUT_BSH = 2, SAS_LAYOUT_BNSD = 3,
        SAS_LAYOUT_PA_ND = 4 };
-enum { SAS_DTYPE_BF16 = 0, SAS_DTYPE_FP16 = 1 };
+enum { SAS_DTYPE_BF16 = 0, SAS_DTYPE_FP16 = 1, SAS_DTYPE_F32 = 2 /* norm weights only */ };
 /* Scenario (api.py:196-202): 1 = SWA, 2 = CFA (dense compressed), 3 = SCFA (top-k). */
 enum { SAS_SCENARIO_SWA = 1, SAS_SCENARIO_CFA = 2, SAS_SCENARIO_SCFA = 3 };
 
@@ -246,6 +250,51 @@ int sas_kv_append(void* pool, int32_t num_blocks, int32_t block_size, int32_t ro
                   const int32_t* block_table, int32_t table_len, const void* rows,
                   const int32_t* cu_new, const int32_t* start_pos, int32_t batch,
                   int32_t total_new, int32_t* err, void* stream);
+
+/* ---- norm and rotation of rows ---- */
+
+#define SAS_MAX_ROW_DIM 1024
+
+/* What happens to a row x[0 .. head_dim): its first norm_dim columns are
+ * multiplied by rsqrt(mean of their squares + eps) and by norm_weight, then
+ * its last rope_dim columns are rotated by the angles of its position.  fp32
+ * inside, rounded once.  norm_dim = 0: no norm; rope_dim = 0: no rotation. */
+typedef struct SasRowTransform {
+  const float* cos;         /* [device] [table_rows, rope_dim / 2], 16-byte aligned       */
+  const float* sin;         /* [device] the same                                          */
+  const void* norm_weight;  /* [device] [norm_dim], 16-byte aligned; NULL = ones          */
+  int32_t table_rows;       /* positions the tables hold                                  */
+  int32_t head_dim;         /* columns: a multiple of 8 up to SAS_MAX_ROW_DIM             */
+  int32_t norm_dim;         /* a multiple of 8 up to head_dim                             */
+  int32_t rope_dim;         /* a multiple of 16 up to head_dim                            */
+  int32_t dtype;            /* of the rows: SAS_DTYPE_BF16 / FP16                         */
+  int32_t weight_dtype;     /* SAS_DTYPE_F32 or the rows' dtype                           */
+  int32_t interleaved;      /* pairs (2 i, 2 i + 1), else (i, i + rope_dim / 2)           */
+  int32_t inverse;          /* rotate by the negative angles                              */
+  float eps;
+} SasRowTransform;
+
+/* Rows x[t, h] of `tokens` x `heads` (strides in elements, multiples of 8;
+ * x and out 16-byte aligned; out == x with the same strides works in place)
+ * into out[t, h], rotated at positions[t] ([device], int32 or, with
+ * positions_i64, int64; may be NULL without rotation).  The rows of a token
+ * whose position is outside the tables become zeros, recorded in the optional
+ * err word [device] int32[4] (site 52, detail = token, head). */
+int sas_norm_rope(const SasRowTransform* transform, const void* x, int64_t x_stride_token,
+                  int64_t x_stride_head, void* out, int64_t out_stride_token,
+                  int64_t out_stride_head, int32_t tokens, int32_t heads, const void* positions,
+                  int32_t positions_i64, int32_t* err, void* stream);
+
+/* sas_kv_append with the transform on the way: the row at logical position p
+ * of its sequence is rotated at position p * cmp_ratio.  Rows outside
+ * [cu_new[0], cu_new[batch]) belong to no sequence and are left out.  A row
+ * whose page is unmapped (site 50) or whose rotation position is past the
+ * tables (site 51) is skipped and recorded in err (detail = row, batch). */
+int sas_kv_append_norm_rope(const SasRowTransform* transform, void* pool, int32_t num_blocks,
+                            int32_t block_size, const int32_t* block_table, int32_t table_len,
+                            const void* new_rows, const int32_t* cu_new, const int32_t* start_pos,
+                            int32_t batch, int32_t total_new, int32_t cmp_ratio, int32_t* err,
+                            void* stream);
 
 /* ---- B200 work plan (host) ---- */
 

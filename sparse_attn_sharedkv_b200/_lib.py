@@ -18,11 +18,12 @@ SAS_OK = 0
 ERRORS = {1: "SAS_ERR_INVALID", 2: "SAS_ERR_UNSUPPORTED", 3: "SAS_ERR_CUDA",
           4: "SAS_ERR_SCHEDULE", 5: "SAS_ERR_WORKSPACE", 6: "SAS_ERR_DEVICE"}
 LAYOUTS = {"BSND": 0, "TND": 1, "BSH": 2, "BNSD": 3, "PA_ND": 4}
-DTYPE_BF16, DTYPE_FP16 = 0, 1
+DTYPE_BF16, DTYPE_FP16, DTYPE_F32 = 0, 1, 2
 SCENARIO_SWA, SCENARIO_CFA, SCENARIO_SCFA = 1, 2, 3
 PHASE_ATTN, PHASE_COMBINE, PHASE_ALL = 1, 2, 3
 SAS_META_SIZE = 1024
 SAS_NOALLOC_SCRATCH_BYTES = 16 << 20
+SAS_MAX_ROW_DIM = 1024
 SAS_AIC_CORE_NUM = 36
 SAS_AIV_CORE_NUM = 72
 SAS_FA_METADATA_SIZE = 8
@@ -84,6 +85,15 @@ class SasPlanInfo(C.Structure):
     ]
 
 
+class SasRowTransform(C.Structure):
+    _fields_ = [
+        ("cos", C.c_void_p), ("sin", C.c_void_p), ("norm_weight", C.c_void_p),
+        ("table_rows", C.c_int32), ("head_dim", C.c_int32), ("norm_dim", C.c_int32),
+        ("rope_dim", C.c_int32), ("dtype", C.c_int32), ("weight_dtype", C.c_int32),
+        ("interleaved", C.c_int32), ("inverse", C.c_int32), ("eps", C.c_float),
+    ]
+
+
 # Exported symbols and their prototypes (must match include/sas.h).
 PROTOTYPES = {
     "sas_metadata": (C.c_int, [C.POINTER(SasMetaParams), _i32p, C.c_size_t]),
@@ -106,6 +116,13 @@ PROTOTYPES = {
     "sas_kv_append": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                 C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                 C.c_int32, C.c_void_p, C.c_void_p]),
+    "sas_norm_rope": (C.c_int, [C.POINTER(SasRowTransform), C.c_void_p, C.c_int64, C.c_int64,
+                                C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32,
+                                C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
+    "sas_kv_append_norm_rope": (C.c_int, [C.POINTER(SasRowTransform), C.c_void_p, C.c_int32,
+                                          C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
+                                          C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                          C.c_int32, C.c_void_p, C.c_void_p]),
     "sas_combine": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
                               C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                               C.c_void_p, C.c_void_p]),

@@ -9,8 +9,12 @@ reference has no device writer (its tests pack caches on the host), so this
 op has no reference signature; it follows the operator's own conventions
 (TND ``cu_seqlens`` for the new rows, int32 tables with -1 = unmapped).
 
-Runs ``sas_kv_append`` from ``libsas.so`` on the caller's stream; there is no
-CPU fallback.
+``append_paged_kv`` copies the rows as they are; ``append_paged_kv_norm_rope``
+norms and rotates them on the way (``rope.norm_rope`` is the same transform
+for the query heads).
+
+Runs ``sas_kv_append`` / ``sas_kv_append_norm_rope`` from ``libsas.so`` on the
+caller's stream; there is no CPU fallback.
 """
 
 from __future__ import annotations
@@ -21,6 +25,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .rope import row_transform
 
 
 def append_paged_kv(kv_pool: torch.Tensor, block_table: torch.Tensor, new_rows: torch.Tensor,
@@ -61,6 +66,67 @@ def append_paged_kv(kv_pool: torch.Tensor, block_table: torch.Tensor, new_rows: 
         D * kv_pool.element_size(), C.c_void_p(bt.data_ptr()), bt.shape[1],
         C.c_void_p(new_rows.data_ptr()), C.c_void_p(cu.data_ptr()), C.c_void_p(sp.data_ptr()),
         B, total, C.c_void_p(err.data_ptr() if err is not None else 0), C.c_void_p(stream)))
+    if err is not None:
+        e = err.tolist()
+        return e if e[0] != 0 else None
+    return None
+
+
+def append_paged_kv_norm_rope(kv_pool: torch.Tensor, block_table: torch.Tensor,
+                              new_rows: torch.Tensor, cu_seqlens_new: torch.Tensor,
+                              start_pos: torch.Tensor, cos: Optional[torch.Tensor] = None,
+                              sin: Optional[torch.Tensor] = None, *, norm_dim: int = 0,
+                              norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                              interleaved: bool = True, cmp_ratio: int = 1,
+                              check_errors: bool = False) -> Optional[list]:
+    """``append_paged_kv`` with each row normed over its first ``norm_dim`` columns and
+    its last ``rope_dim`` columns rotated on the way into ``kv_pool``.
+
+    The pool, table, ``cu_seqlens_new`` and ``start_pos`` are ``append_paged_kv``'s; cos,
+    sin, norm_dim, norm_weight, eps and interleaved are ``rope.norm_rope``'s.  The row at
+    logical position p of its sequence is rotated at position ``p * cmp_ratio`` (the first
+    token of those that a row of a ratio-compressed cache stands for).  new_rows
+    [T_new, 1, D] or [T_new, D]; rows at or past ``cu_seqlens_new[-1]`` belong to no
+    sequence and are left out.
+
+    Rows on an unmapped page or past the tables are skipped; two rows of one call must not
+    share a slot.  With ``check_errors`` the call synchronises and returns the device error
+    record ``[code, site, row, batch]`` if any row was skipped (else None).
+    """
+    dev = kv_pool.device
+    if dev.type != "cuda" or new_rows.device != dev:
+        raise RuntimeError("kv_pool and new_rows must be on one CUDA (sm_100a) device")
+    if kv_pool.dim() not in (3, 4) or (kv_pool.dim() == 4 and kv_pool.shape[2] != 1):
+        raise ValueError("kv_pool must be [blocks, block_size, 1, D]")
+    D = kv_pool.shape[-1]
+    if new_rows.dtype != kv_pool.dtype or new_rows.shape[-1] != D:
+        raise ValueError("new_rows must have the pool's dtype and last dim")
+    if not kv_pool.is_contiguous() or not new_rows.is_contiguous():
+        raise ValueError("kv_pool and new_rows must be contiguous")
+    if kv_pool.shape[1] < 1:
+        raise ValueError("block_size must be >= 1")
+    if block_table.dim() != 2 or block_table.shape[0] < 1:
+        raise ValueError("block_table must be [B, table_len] with B >= 1")
+    if cmp_ratio < 1:
+        raise ValueError(f"cmp_ratio must be >= 1 (got {cmp_ratio})")
+    B = block_table.shape[0]
+    if cu_seqlens_new.numel() != B + 1 or start_pos.numel() != B:
+        raise ValueError("cu_seqlens_new must have B + 1 entries and start_pos B")
+    tr = row_transform(kv_pool.dtype, dev, D, cos, sin, int(norm_dim), norm_weight, eps,
+                       interleaved, False)
+    total = new_rows.numel() // D
+    if total == 0:
+        return None
+    bt = block_table.to(device=dev, dtype=torch.int32).contiguous()
+    cu = cu_seqlens_new.to(device=dev, dtype=torch.int32).contiguous()
+    sp = start_pos.to(device=dev, dtype=torch.int32).contiguous()
+    err = torch.zeros(4, dtype=torch.int32, device=dev) if check_errors else None
+    with torch.cuda.device(dev):
+        _lib.check("sas_kv_append_norm_rope", _lib.lib().sas_kv_append_norm_rope(
+            C.byref(tr), kv_pool.data_ptr(), kv_pool.shape[0], kv_pool.shape[1], bt.data_ptr(),
+            bt.shape[1], new_rows.data_ptr(), cu.data_ptr(), sp.data_ptr(), B, total,
+            int(cmp_ratio), err.data_ptr() if err is not None else None,
+            torch.cuda.current_stream(dev).cuda_stream))
     if err is not None:
         e = err.tolist()
         return e if e[0] != 0 else None
