@@ -33,6 +33,10 @@
  *       the norm and rotation of query heads and of key rows on their way into
  *       a paged cache, the step before the path; the reference takes both
  *       already transformed (api.py:129-153).
+ *   sas_index_scores / sas_topk_select
+ *       the scores and the selection that make the top-k index lists
+ *       (cmp_sparse_indices) the path takes; the reference's tests draw them at
+ *       random (golden.py:411-473).
  *   sas_error_string / sas_version
  *       error reporting in place of the reference's Python asserts
  *       (api.py:187-191, 279-282).
@@ -295,6 +299,54 @@ int sas_kv_append_norm_rope(const SasRowTransform* transform, void* pool, int32_
                             const void* new_rows, const int32_t* cu_new, const int32_t* start_pos,
                             int32_t batch, int32_t total_new, int32_t cmp_ratio, int32_t* err,
                             void* stream);
+
+/* ---- selection of key positions ---- */
+
+#define SAS_MAX_INDEX_HEADS 128
+#define SAS_MAX_INDEX_DIM 128
+
+/* Index scores of the tokens [first_token, first_token + num_tokens) against
+ * the paged index keys of their sequences:
+ *   scores[t, j] = sum_h weights[t, h] * relu(q[t, h, :] . key[j, :])
+ * for j below the keys that token s of its sequence sees, len = (kv_len -
+ * q_len + s + 1) / cmp_ratio (rounded down, cut to [0, num_keys]), -inf for
+ * the others; a key whose page is unmapped or past the table scores -inf, and
+ * a page id past the pool is recorded in err (site 53, detail = page,
+ * batch).  Tokens of no sequence see no key. */
+typedef struct SasIndexParams {
+  const void* q;                /* [device] [total_tokens, H, D], 16-byte aligned       */
+  const float* weights;         /* [device] [total_tokens, H]                           */
+  const void* key_pool;         /* [device] [num_blocks, block_size, 1, D], 16-byte
+                                   aligned                                              */
+  const int32_t* block_table;   /* [device] [batch, table_len]                          */
+  const int32_t* cu_seqlens_q;  /* [device] [batch + 1]; may be NULL for BSND           */
+  const int32_t* kv_len;        /* [device] [batch] uncompressed lengths (seqused_kv)   */
+  float* scores;                /* [device] [num_tokens, score_stride]                  */
+  int32_t* lengths;             /* [device] optional [num_tokens]: len of each token    */
+  int32_t* err;                 /* [device] optional int32[4] error record              */
+  int32_t batch;
+  int32_t total_tokens;         /* T (TND) or batch * max_q_len (BSND)                  */
+  int32_t max_q_len;            /* BSND: S; TND: 0                                      */
+  int32_t num_heads;            /* 1 .. SAS_MAX_INDEX_HEADS                             */
+  int32_t head_dim;             /* a multiple of 8 up to SAS_MAX_INDEX_DIM              */
+  int32_t dtype;                /* of q and the keys: SAS_DTYPE_BF16 / FP16             */
+  int32_t block_size, num_blocks, table_len;
+  int32_t cmp_ratio;            /* tokens a key stands for (>= 1)                       */
+  int32_t num_keys;             /* columns of scores                                    */
+  int32_t first_token, num_tokens;
+  int32_t fill;                 /* 0: the columns at and past len are left as they are  */
+  int64_t score_stride;         /* row stride of scores in elements (>= num_keys)       */
+} SasIndexParams;
+
+int sas_index_scores(const SasIndexParams* params, void* stream);
+
+/* For each of `rows` rows of scores ([device], row stride in elements) the
+ * positions of its topk largest scores among the first lengths[row] (all
+ * num_keys with lengths NULL), ties to the lower position, in ascending order
+ * and -1 behind them, into indices [device] [rows, topk].  -inf is never
+ * selected, NaN ranks above +inf. */
+int sas_topk_select(const float* scores, int64_t score_stride, const int32_t* lengths,
+                    int32_t rows, int32_t num_keys, int32_t topk, int32_t* indices, void* stream);
 
 /* ---- B200 work plan (host) ---- */
 

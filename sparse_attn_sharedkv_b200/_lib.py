@@ -24,6 +24,8 @@ PHASE_ATTN, PHASE_COMBINE, PHASE_ALL = 1, 2, 3
 SAS_META_SIZE = 1024
 SAS_NOALLOC_SCRATCH_BYTES = 16 << 20
 SAS_MAX_ROW_DIM = 1024
+SAS_MAX_INDEX_HEADS = 128
+SAS_MAX_INDEX_DIM = 128
 SAS_AIC_CORE_NUM = 36
 SAS_AIV_CORE_NUM = 72
 SAS_FA_METADATA_SIZE = 8
@@ -94,6 +96,19 @@ class SasRowTransform(C.Structure):
     ]
 
 
+class SasIndexParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("weights", C.c_void_p), ("key_pool", C.c_void_p),
+        ("block_table", C.c_void_p), ("cu_seqlens_q", C.c_void_p), ("kv_len", C.c_void_p),
+        ("scores", C.c_void_p), ("lengths", C.c_void_p), ("err", C.c_void_p),
+        ("batch", C.c_int32), ("total_tokens", C.c_int32), ("max_q_len", C.c_int32),
+        ("num_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32),
+        ("block_size", C.c_int32), ("num_blocks", C.c_int32), ("table_len", C.c_int32),
+        ("cmp_ratio", C.c_int32), ("num_keys", C.c_int32), ("first_token", C.c_int32),
+        ("num_tokens", C.c_int32), ("fill", C.c_int32), ("score_stride", C.c_int64),
+    ]
+
+
 # Exported symbols and their prototypes (must match include/sas.h).
 PROTOTYPES = {
     "sas_metadata": (C.c_int, [C.POINTER(SasMetaParams), _i32p, C.c_size_t]),
@@ -123,6 +138,9 @@ PROTOTYPES = {
                                           C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
                                           C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
                                           C.c_int32, C.c_void_p, C.c_void_p]),
+    "sas_index_scores": (C.c_int, [C.POINTER(SasIndexParams), C.c_void_p]),
+    "sas_topk_select": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int32,
+                                  C.c_int32, C.c_void_p, C.c_void_p]),
     "sas_combine": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
                               C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                               C.c_void_p, C.c_void_p]),
