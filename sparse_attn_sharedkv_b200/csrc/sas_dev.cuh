@@ -159,6 +159,97 @@ __device__ __forceinline__ void mma_ws(uint32_t d_tmem, uint64_t a_desc, uint64_
       : "memory");
 }
 
+// ---- CTA pairs (clusters of two) ----
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t peer_addr(uint32_t a, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+
+// Arrival on a barrier of the other CTA of the pair (shared::cluster
+// address).  Relaxed: every forwarded phase guards shared memory or TMEM that
+// was complete before the arrival (generic stores fenced to the async proxy,
+// TMEM stores waited), so the arrival only signals.
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
+
+// Arrival with `bytes` of expected transactions on a barrier of the leader
+// (shared::cluster address).  Release when the caller's own shared-memory
+// writes (cp.async rows) must be visible before the phase completes.
+__device__ __forceinline__ void arrive_tx_cluster(uint32_t cluster_bar, uint32_t bytes,
+                                                  bool release) {
+  if (release)
+    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(
+                     cluster_bar),
+                 "r"(bytes)
+                 : "memory");
+  else
+    asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(
+                     cluster_bar),
+                 "r"(bytes)
+                 : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+
+// 2D tiled TMA load into this CTA's shared memory whose transactions complete
+// on the barrier `bar` of the CTA pair's leader (shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                                 uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+// tile::gather4 of rows y0..y3 (column block x) into 4 consecutive 128-byte
+// rows at dst, completing on the leader's barrier `bar`.
+__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap* map, int x,
+                                                 int y0, int y1, int y2, int y3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::"
+      "complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y0), "r"(y1), "r"(y2), "r"(y3), "r"(bar)
+      : "memory");
+}
+
+// D[tmem] (+)= A[smem] * B[smem] over the CTA pair (half of A's rows and half
+// of B's columns in each CTA; D in each CTA's TMEM: M = 128: 64 rows, columns
+// [0, N/2) on lanes 0-63 and [N/2, N) on lanes 64-127; M = 256: 128 rows by N
+// columns).  Issued by the leader CTA only.
+__device__ __forceinline__ void mma2(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                     uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrives once on the barrier at the same offset in both CTAs when every MMA
+// the leader issued so far has completed.
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
 // 32 consecutive 32-bit columns of this warp's 32 TMEM lanes.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(

@@ -11,27 +11,36 @@
 //
 // Work.  A group is up to 256 / Hp consecutive tokens of one sequence (Hp:
 // the heads, padded to 16, 32, 64 or 128), so that the (token, head) pairs of
-// a group are the N <= 256 columns of one tcgen05.mma; its M = 128 rows are a
-// tile of 128 keys.  With keys in the rows, a thread of the epilogue owns one
-// key and sums over heads along its own TMEM lane, without exchanging
-// anything; the weights of its columns stay in registers over all the key
-// tiles of a group.  An item is a group and a span of its key tiles; a
-// persistent block per SM takes every gridDim-th item.  Tiles that no token of
-// the group sees are filled with -inf without loads.
+// a group are the N <= 256 columns of one MMA; its M = 256 rows are a tile of
+// 256 keys, 128 in each CTA of a pair (tcgen05.mma.cta_group::2).  With keys
+// in the rows, a thread of the epilogue owns one key and sums over heads along
+// its own TMEM lane, without exchanging anything; the weights of its columns
+// stay in registers over all the key tiles of a group.  The pair halves what
+// the queries take of each SM's shared memory (room for five key stages beside
+// two query buffers) and the operand reads of each MMA.  An item is a group
+// and a span of its key tiles; a persistent pair takes every num_pairs-th
+// item.  Tiles that no token of the group sees are filled with -inf without
+// loads.
 //
-// Warp roles (384 threads, one block per SM):
-//   0      keys: page lookup of a tile, TMA into a ring of stages (boxes of a
-//          page's rows where the page size allows, tile::gather4 else)
-//   1      MMA issue (one lane), accumulators alternating between two halves
-//          of TMEM
-//   2      queries of the next item into the other of two buffers; TMEM
+// Warp roles in each CTA (384 threads, one CTA per SM):
+//   0, 3   keys, every other tile each: page lookup, TMA into a ring of stages
+//          (boxes of a page's rows where the page size allows, tile::gather4
+//          else)
+//   1      CTA 0: MMA issue (one lane), accumulators alternating between two
+//          halves of TMEM
+//   2      items: the group of the next item, its queries into the other of
+//          two buffers, its weights; the -inf fill; TMEM
 //   4-11   epilogue: warpgroup g takes columns 128 g .. 128 g + 127 of each
 //          accumulator: relu, weight, sum over heads, mask, store
 //
-// Every wait is bounded (~2 s): on timeout the thread records an error and
-// raises the block's abort flag, on which every role leaves its loop.
+// TMA loads of both CTAs complete on the leader's barriers; the leader's
+// commits arrive in both CTAs; CTA 1's epilogue releases accumulators on the
+// leader's barrier.  Every wait is bounded (~2 s): on timeout the thread
+// records an error and raises its CTA's abort flag, on which every role leaves
+// its loop; both CTAs meet at the final cluster barriers.
 
 #include <math_constants.h>
+#include <stddef.h>
 
 #include "sas_dev.cuh"
 
@@ -39,51 +48,70 @@ namespace sas {
 namespace {
 
 constexpr int kIxThreads = 384;
-constexpr int kIxKeys = 128;           // keys of a tile (M)
-constexpr int kIxCols = 256;           // (token, head) columns of a group (N)
-constexpr int kIxHalf = kIxCols / 2;   // columns of an epilogue warpgroup
+constexpr int kIxKeys = 128;               // keys of a CTA's tile
+constexpr int kIxTile = 2 * kIxKeys;       // keys of the pair's tile (M)
+constexpr int kIxCols = 256;               // (token, head) columns of a group (N)
+constexpr int kIxHalf = kIxCols / 2;       // columns of an epilogue warpgroup
+constexpr int kIxTokens = kIxCols / 16;    // tokens of a group at most
 constexpr int kIxMaxStages = 8;
-constexpr int kIxBits = 16;            // tiles whose page bits are kept
-constexpr int kIxQChunk = kIxCols * 128;   // 64 dims of a group's columns
-constexpr int kIxKChunk = kIxKeys * 128;   // 64 dims of a key tile
+constexpr int kIxBits = 16;                // tiles whose page bits are kept
+constexpr int kIxItems = 4;                // items described ahead
+constexpr int kIxQChunk = kIxHalf * 128;   // 64 dims of a CTA's half of the columns
+constexpr int kIxKChunk = kIxKeys * 128;   // 64 dims of a CTA's key tile
 constexpr int kIxSmem = 232448;            // the per-block opt-in maximum
 
 // Registers of the loading and issuing warpgroup and of an epilogue one: 88 +
 // 2 x 208 = 3 x 168, the launch's share of 384 threads.
 constexpr int kIxRegsLoad = 88, kIxRegsEpi = 208;
 
+// An item as its roles need it: tokens tok0 .. tok0 + live (relative to the
+// call's first), of sequence `batch`; key tiles [t0, tc) are computed.
+struct IxInfo {
+  int tok0, live, batch, most, t0, tc, fill, pad;
+  int len[kIxTokens];  // keys that each token sees
+};
+
 struct IxCtl {
-  uint64_t q_full[2], q_empty[2];
+  uint64_t q_full[2], q_empty[2];  // full: leader, one arrival per CTA and the bytes of both
   uint64_t k_full[kIxMaxStages], k_empty[kIxMaxStages];
-  // Two arrivals: the issuing thread (for the page bits it has seen written)
-  // and the commit of the tile's MMAs.
-  uint64_t acc_full[2];
-  uint64_t acc_empty[2];
+  uint64_t acc_full[2], acc_empty[2];  // empty: leader, the epilogue warps of both CTAs
+  uint64_t item_full[kIxItems], item_empty[kIxItems];
+  uint64_t w_full, w_empty;
+  uint64_t bits_full[kIxBits];
   uint64_t drain;
   uint32_t tmem_base;
   volatile int abort;
-  // Byte i of a tile: bit r set when key 4 i + r has a page.  The slot of
-  // tile n is written again for tile n + kIxBits, after the MMAs of tile n +
-  // kIxBits - stages, whose accumulator the epilogue released behind tile
-  // n + kIxBits - stages - 3 >= n.
-  uint8_t bits[kIxBits][32];
+  uint8_t issued[kIxMaxStages];  // 1 + parity of the stage's last load, 0 before the first
+  // Bit r of byte i of a tile: key 8 i + r has a page.  The slot of tile n is
+  // written again for tile n + kIxBits, after the MMAs of tile n + kIxBits -
+  // stages, whose accumulator the epilogue released behind tile n + kIxBits -
+  // stages - 3 >= n.
+  uint8_t bits[kIxBits][16];
+  IxInfo items[kIxItems];
+  alignas(16) float w[kIxCols];  // read as 16-byte vectors
 };
+static_assert(offsetof(IxCtl, w) % 16 == 0 && alignof(IxCtl) == 16, "vector reads of w");
 static_assert(kIxBits >= kIxMaxStages + 3, "page bits are kept long enough");
+
+// Shared memory: two query buffers, the key stages, control.
+template <int kChunks>
+struct IxSmem {
+  static constexpr int kQ = kChunks * kIxQChunk;
+  static constexpr int kFit = (kIxSmem - (int)sizeof(IxCtl) - 2 * kQ) / (kChunks * kIxKChunk);
+  static constexpr int kStages = kFit < kIxMaxStages ? kFit : kIxMaxStages;
+  static constexpr int kCtl = 2 * kQ + kStages * kChunks * kIxKChunk;
+};
+static_assert(IxSmem<1>::kCtl % 16 == 0 && IxSmem<2>::kCtl % 16 == 0, "control block alignment");
+static_assert(IxSmem<2>::kStages == 5, "five stages of 128 keys by 128 dims fit");
 
 struct IxArgs {
   SasIndexParams p;
-  int32_t hp, tq;              // padded heads, tokens of a group
+  int32_t tq_shift;            // log2 of the tokens of a group
   int32_t groups;              // groups of the call (some may be empty)
   int32_t tiles, span_tiles, spans;
-  int32_t box_rows;            // rows of a key box, 0: tile::gather4
+  int32_t box_shift;           // log2 of the rows of a key box, 0: tile::gather4
   int32_t no_row;              // row past the pool: reads as zeros
-  int32_t chunks, stages;
-};
-
-// Group g: tokens tok0 .. tok0 + live of the call (relative to first_token),
-// of sequence `batch` (p.batch: of none), whose tokens start at `start`.
-struct IxGroup {
-  int tok0, live, batch, start, q_len, kv;
+  uint32_t idesc;              // MMA instruction without its N
 };
 
 __device__ __forceinline__ int ix_start(const SasIndexParams& p, int b) {
@@ -96,13 +124,18 @@ __device__ __forceinline__ int ix_local(const SasIndexParams& p, int b) {
   return min(max(ix_start(p, b) - p.first_token, 0), p.num_tokens);
 }
 
+// Item `item` by a whole warp, lane i with the length of token i in *len.
 // Sequence b owns the groups from (local(b) + b (tq - 1)) / tq on: at least
-// ceil(tokens / tq) of them, without a scan over the lengths before it.  The
-// tokens behind the last sequence are those of a sequence p.batch.  Called by
-// whole warps: 32 probes a step.
-__device__ __forceinline__ IxGroup ix_group(const IxArgs& a, int g, int lane) {
+// ceil(tokens / tq) of them, without a scan over the lengths before it; the
+// group's sequence is searched with 32 probes a step.  The tokens behind the
+// last sequence are those of a sequence p.batch that sees no key.
+__device__ __forceinline__ IxInfo ix_item(const IxArgs& a, int item, int lane, int* t1) {
   const SasIndexParams& p = a.p;
-  auto first = [&](int b) { return (int)(((int64_t)ix_local(p, b) + (int64_t)b * (a.tq - 1)) / a.tq); };
+  const int tq = 1 << a.tq_shift;
+  const int g = item / a.spans;
+  auto first = [&](int b) {
+    return (int)(((int64_t)ix_local(p, b) + (int64_t)b * (tq - 1)) >> a.tq_shift);
+  };
   int lo = 0, hi = p.batch;
   while (lo < hi) {
     const int step = (hi - lo + 32) / 32;
@@ -112,67 +145,36 @@ __device__ __forceinline__ IxGroup ix_group(const IxArgs& a, int g, int lane) {
     lo += (n - 1) * step;
     hi = min(hi, lo + step - 1);
   }
-  IxGroup r;
-  r.batch = lo;
-  r.start = lo < p.batch || p.max_q_len == 0 ? ix_start(p, lo) : p.total_tokens;
-  const int begin = ix_local(p, lo);
+  const int begin = ix_local(p, lo), f = first(lo);
   const int end = lo < p.batch ? ix_local(p, lo + 1) : p.num_tokens;
-  const int64_t t0 = (int64_t)begin + (int64_t)(g - first(lo)) * a.tq;
-  r.tok0 = (int)(t0 < end ? t0 : end);
-  r.live = g < first(lo) ? 0 : max(0, min(a.tq, end - r.tok0));
-  r.q_len = 0;
-  r.kv = 0;
-  if (lo < p.batch) {
-    r.q_len = p.cu_seqlens_q ? __ldg(p.cu_seqlens_q + lo + 1) - __ldg(p.cu_seqlens_q + lo)
-                             : p.max_q_len;
-    r.kv = __ldg(p.kv_len + lo);
+  const int64_t tok = (int64_t)begin + (int64_t)(g - f) * tq;
+  IxInfo r;
+  r.batch = lo;
+  r.tok0 = (int)(tok < end ? tok : end);
+  r.live = g < f ? 0 : max(0, min(tq, end - r.tok0));
+  r.len[0] = 0;
+  if (lo < p.batch && lane < r.live) {
+    const int start = ix_start(p, lo);
+    const int q_len =
+        p.cu_seqlens_q ? __ldg(p.cu_seqlens_q + lo + 1) - __ldg(p.cu_seqlens_q + lo) : p.max_q_len;
+    const int s = p.first_token + r.tok0 + lane - start;
+    if (s >= 0 && s < q_len) {
+      const int64_t n = floordiv((int64_t)__ldg(p.kv_len + lo) - q_len + s + 1, p.cmp_ratio);
+      r.len[0] = n < 0 ? 0 : n > p.num_keys ? p.num_keys : (int)n;
+    }
   }
+  r.most = __reduce_max_sync(0xffffffffu, r.len[0]);
+  r.t0 = (item - g * a.spans) * a.span_tiles;
+  *t1 = min(r.t0 + a.span_tiles, a.tiles);
+  r.tc = max(r.t0, min(*t1, (r.most + kIxTile - 1) / kIxTile));
   return r;
 }
 
-// Keys that token `i` of the group sees.
-__device__ __forceinline__ int ix_len(const SasIndexParams& p, const IxGroup& g, int i) {
-  const int s = p.first_token + g.tok0 + i - g.start;
-  if (i >= g.live || g.batch >= p.batch || s < 0 || s >= g.q_len) return 0;
-  const int64_t n = floordiv((int64_t)g.kv - g.q_len + s + 1, p.cmp_ratio);
-  return n < 0 ? 0 : n > p.num_keys ? p.num_keys : (int)n;
-}
-
-// Item: a group and its key tiles [t0, t1), computed up to tc, filled behind.
-struct IxItem {
-  IxGroup g;
-  int len;   // of token `lane`
-  int most;  // the longest of the group
-  int t0, t1, tc;
-};
-
-__device__ __forceinline__ IxItem ix_item(const IxArgs& a, int item, int lane) {
-  IxItem r;
-  const int gi = item / a.spans;
-  r.g = ix_group(a, gi, lane);
-  r.len = ix_len(a.p, r.g, lane);
-  r.most = __reduce_max_sync(0xffffffffu, r.len);
-  r.t0 = (item - gi * a.spans) * a.span_tiles;
-  r.t1 = min(r.t0 + a.span_tiles, a.tiles);
-  r.tc = max(r.t0, min(r.t1, (r.most + kIxKeys - 1) / kIxKeys));
-  return r;
-}
-
-__device__ __forceinline__ void ix_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                       uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int x,
+                                                 int y, int z, uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y,
-                                            int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
@@ -184,6 +186,25 @@ __device__ __forceinline__ float relu_nan(uint32_t bits) {
   return y;
 }
 
+// Pairs of fp32 in one 64-bit register, for the packed FMA.
+__device__ __forceinline__ uint64_t pack_f32(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+__device__ __forceinline__ float sum_f32(uint64_t a) {
+  float x, y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a));
+  return x + y;
+}
+
 // Wait for copies or MMAs already issued, abort or not; bounded.
 __device__ __forceinline__ void ix_settle(uint64_t* bar, uint32_t parity) {
   const long long t0 = clock64();
@@ -191,271 +212,439 @@ __device__ __forceinline__ void ix_settle(uint64_t* bar, uint32_t parity) {
   }
 }
 
-// Row in the pool of logical key position `pos`, no_row without a page or
-// where no token of the group looks.
-__device__ __forceinline__ int ix_row(const IxArgs& a, int batch, int pos, int most) {
+// Wait by a whole warp.
+__device__ __forceinline__ bool ix_wait(IxCtl& ctl, uint64_t* bar, int parity, int32_t* err,
+                                        int site) {
+  return __all_sync(0xffffffffu, wait_bar(&ctl, bar, (uint32_t)parity, err, site));
+}
+
+// The next item of a role's warp; it may be overwritten once the warp has
+// arrived on its item_empty.
+__device__ __forceinline__ const IxInfo* ix_next(IxCtl& ctl, int i, int32_t* err, int site) {
+  const int slot = i % kIxItems;
+  if (!ix_wait(ctl, &ctl.item_full[slot], (i / kIxItems) & 1, err, site)) return nullptr;
+  return &ctl.items[slot];
+}
+
+__device__ __forceinline__ void ix_done(IxCtl& ctl, int i, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(smem_addr(&ctl.item_empty[i % kIxItems]));
+}
+
+// Pages of logical key positions that advance by a fixed step: one division
+// at the start.
+struct IxPage {
+  int lb, off;  // page of the table, row inside it
+  __device__ __forceinline__ void start(const SasIndexParams& p, int pos) {
+    lb = pos / p.block_size;
+    off = pos - lb * p.block_size;
+  }
+  __device__ __forceinline__ void advance(const SasIndexParams& p, int pages, int rows) {
+    lb += pages;
+    off += rows;
+    if (off >= p.block_size) {
+      off -= p.block_size;
+      ++lb;
+    }
+  }
+  // Page id as the table has it (-1 past the table).
+  __device__ __forceinline__ int id(const SasIndexParams& p, const int32_t* table) const {
+    return lb < p.table_len ? __ldg(table + lb) : -1;
+  }
+};
+
+// Row in the pool, no_row without a page.
+__device__ __forceinline__ int ix_row(const IxArgs& a, int id, int off) {
+  if (id >= a.p.num_blocks) record_error(a.p.err, SAS_ERR_DEVICE, 53, id);
+  return id < 0 || id >= a.p.num_blocks ? a.no_row : id * a.p.block_size + off;
+}
+
+// Keys of the tiles n % 2 == half of the pair's tiles, n counted over its
+// items: page ids are read two tiles ahead of their use, behind the wait for
+// a stage.
+template <int kChunks>
+__device__ __forceinline__ void ix_keys(const IxArgs& a, IxCtl& ctl, uint32_t sK, int count,
+                                        const CUtensorMap* tm_k, int half, int rank, int lane) {
+  constexpr int kStages = IxSmem<kChunks>::kStages;
   const SasIndexParams& p = a.p;
-  const int lb = pos / p.block_size;
-  if (pos >= most || lb >= p.table_len) return a.no_row;
-  const int blk = __ldg(p.block_table + (size_t)batch * p.table_len + lb);
-  if (blk >= p.num_blocks) record_error(p.err, SAS_ERR_DEVICE, 53, blk);
-  if (blk < 0 || blk >= p.num_blocks) return a.no_row;
-  return blk * p.block_size + (pos - lb * p.block_size);
+  const bool gather = a.box_shift == 0;
+  const int boxes = gather ? 32 : kIxKeys >> a.box_shift;
+  const int step = gather ? 4 : 1 << a.box_shift;  // rows of a lane
+  const int my_box = a.box_shift > 0 ? (8 * (lane & 15)) >> a.box_shift : 0;
+  const int adv_pages = 2 * kIxTile / p.block_size, adv_rows = 2 * kIxTile % p.block_size;
+  const uint32_t full0 = peer_addr(smem_addr(&ctl.k_full[0]), 0);
+  int n = 0;               // tiles before the item's first
+  int s = half, ph = 1;    // stage and parity of the warp's next tile
+  for (int i = 0; i < count; ++i) {
+    const IxInfo* info = ix_next(ctl, i, p.err, 69);
+    if (info == nullptr) return;
+    const int t0 = info->t0, tc = info->tc, most = info->most;
+    const int32_t* table = p.block_table + (size_t)info->batch * p.table_len;
+    ix_done(ctl, i, lane);
+    if (tc == t0) continue;
+    int t = t0 + ((n ^ half) & 1);
+    int pos = t * kIxTile + rank * kIxKeys + lane * step;
+    IxPage pg;
+    pg.start(p, pos);
+    int id[4];
+    auto read_ids = [&](int tile) {
+      if (!gather) {
+        id[0] = lane < boxes && tile < tc && pos < most ? pg.id(p, table) : -1;
+      } else {
+        IxPage q = pg;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          id[r] = tile < tc && pos + r < most ? q.id(p, table) : -1;
+          q.advance(p, 0, 1);
+        }
+      }
+    };
+    read_ids(t);
+    for (; t < tc; t += 2) {
+      const uint32_t stage = sK + (uint32_t)(s * kChunks * kIxKChunk);
+      const uint32_t bar = full0 + 8u * (uint32_t)s;
+      const int slot = (n + t - t0) % kIxBits;
+      if (!ix_wait(ctl, &ctl.k_empty[s], ph, p.err, 70)) return;
+      int rows[4];
+      if (!gather) {
+        rows[0] = ix_row(a, id[0], pg.off);
+        const uint32_t mapped = __ballot_sync(0xffffffffu, rows[0] != a.no_row);
+        if (lane < 16) ctl.bits[slot][lane] = (mapped >> my_box) & 1 ? 255 : 0;
+      } else {
+        IxPage q = pg;
+        uint32_t four = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          rows[r] = ix_row(a, id[r], q.off);
+          four |= (rows[r] != a.no_row ? 1u : 0u) << r;
+          q.advance(p, 0, 1);
+        }
+        const uint32_t next = __shfl_down_sync(0xffffffffu, four, 1);
+        if ((lane & 1) == 0) ctl.bits[slot][lane >> 1] = (uint8_t)(four | next << 4);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_addr(&ctl.bits_full[slot]));
+        ctl.issued[s] = (uint8_t)(1 + (ph ^ 1));
+        arrive_tx_cluster(bar, (uint32_t)(kChunks * kIxKChunk), false);
+      }
+      __syncwarp();
+      if (lane < boxes) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const uint32_t dst = stage + (uint32_t)(c * kIxKChunk + lane * step * 128);
+          if (gather)
+            tma_gather4_pair(dst, tm_k, c * 64, rows[0], rows[1], rows[2], rows[3], bar);
+          else
+            tma_load_2d_pair(dst, tm_k, c * 64, rows[0], bar);
+        }
+      }
+      s += 2;
+      if (s >= kStages) {
+        s -= kStages;
+        ph ^= 1;
+      }
+      pos += 2 * kIxTile;
+      pg.advance(p, adv_pages, adv_rows);
+      read_ids(t + 2);
+    }
+    n += tc - t0;
+  }
 }
 
 template <int kHp>
-__device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_t tmem, int items) {
+__device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_t tmem, int count,
+                                            int rank) {
   const SasIndexParams& p = a.p;
   constexpr int kTok = kIxHalf / kHp;  // tokens of a warpgroup
   const int tid = threadIdx.x - 128, wg = tid >> 7, lane = tid & 31;
   const int row = tid & 127;
   const uint32_t base = tmem + ((uint32_t)(row & ~31) << 16) + (uint32_t)(wg * kIxHalf);
-  float w[kIxHalf];
+  const uint32_t empty0 = peer_addr(smem_addr(&ctl.acc_empty[0]), 0);
+  uint64_t w[kIxHalf / 2];
 #pragma unroll
-  for (int i = 0; i < kIxHalf; ++i) w[i] = 0.0f;
-  int n = 0;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    if (ctl.abort) break;
-    const IxItem it = ix_item(a, item, lane);
-    const int tok0 = it.g.tok0 + wg * kTok;           // first token of the warpgroup
-    const int live = min(kTok, it.g.live - wg * kTok);  // its tokens, may be <= 0
-    if (it.t0 == 0 && p.lengths != nullptr && tid < it.g.live) p.lengths[it.g.tok0 + tid] = it.len;
-    if (it.tc > it.t0) {
+  for (int i = 0; i < kIxHalf / 2; ++i) w[i] = 0;
+  int n = 0, m = 0;
+  for (int i = 0; i < count; ++i) {
+    const IxInfo* info = ix_next(ctl, i, p.err, 73);
+    if (info == nullptr) return;
+    const int t0 = info->t0, tc = info->tc;
+    const int tok0 = info->tok0 + wg * kTok;           // first token of the warpgroup
+    const int live = min(kTok, info->live - wg * kTok);  // its tokens, may be <= 0
+    int len[kTok];
 #pragma unroll
-      for (int i = 0; i < kIxHalf; ++i) {
-        const int t = i / kHp, h = i % kHp;
-        w[i] = t < live && h < p.num_heads
-                   ? __ldg(p.weights + (size_t)(p.first_token + tok0 + t) * p.num_heads + h)
-                   : 0.0f;
-      }
+    for (int t = 0; t < kTok; ++t) len[t] = info->len[wg * kTok + t];
+    ix_done(ctl, i, lane);
+    if (tc == t0) continue;
+    if (!ix_wait(ctl, &ctl.w_full, m & 1, p.err, 79)) return;
+#pragma unroll
+    for (int c = 0; c < kIxHalf / 4; ++c) {
+      const float4 v = *reinterpret_cast<const float4*>(&ctl.w[wg * kIxHalf + 4 * c]);
+      w[2 * c] = pack_f32(v.x, v.y);
+      w[2 * c + 1] = pack_f32(v.z, v.w);
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_addr(&ctl.w_empty));
+    ++m;
     float* out = p.scores + (size_t)max(tok0, 0) * p.score_stride;
-    bool ok = true;
-    for (int t = it.t0; t < it.tc; ++t, ++n) {
-      const int b = n & 1;
-      if (!__all_sync(0xffffffffu, wait_bar(&ctl, &ctl.acc_full[b], (uint32_t)(n >> 1) & 1, p.err, 73))) {
-        ok = false;
-        break;
-      }
+    for (int t = t0; t < tc; ++t, ++n) {
+      const int b = n & 1, slot = n % kIxBits;
+      if (!ix_wait(ctl, &ctl.acc_full[b], (n >> 1) & 1, p.err, 80) ||
+          !ix_wait(ctl, &ctl.bits_full[slot], (n / kIxBits) & 1, p.err, 81))
+        return;
       tc_fence_after();
-      const int key = t * kIxKeys + row;
-      const bool paged = (ctl.bits[n % kIxBits][row >> 2] >> (row & 3)) & 1;
+      const int key = t * kIxTile + rank * kIxKeys + row;
+      const bool paged = (ctl.bits[slot][row >> 3] >> (row & 7)) & 1;
       const uint32_t acc = base + (uint32_t)(b * kIxCols);
       uint32_t v[2][16];
       if (live > 0) tmem_ld16(acc, v[0]);
-      float s0 = 0.0f, s1 = 0.0f;
+      uint64_t s0 = 0, s1 = 0;
 #pragma unroll
       for (int c = 0; c < kIxHalf / 16; ++c) {
         constexpr int kPieces = kHp / 16;  // 16-column pieces of a token
         const int tok = c / kPieces;
         if (tok < live) {
           tmem_wait_ld();
-          if (c + 1 < kIxHalf / 16 && (c + 1) / kPieces < live) tmem_ld16(acc + 16u * (c + 1), v[(c + 1) & 1]);
+          if (c + 1 < kIxHalf / 16 && (c + 1) / kPieces < live)
+            tmem_ld16(acc + 16u * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            s0 = fmaf(w[16 * c + i], relu_nan(v[c & 1][i]), s0);
-            s1 = fmaf(w[16 * c + i + 1], relu_nan(v[c & 1][i + 1]), s1);
+          for (int k = 0; k < 16; k += 4) {
+            const uint32_t* x = &v[c & 1][k];
+            s0 = fma2(w[8 * c + k / 2], pack_f32(relu_nan(x[0]), relu_nan(x[1])), s0);
+            s1 = fma2(w[8 * c + k / 2 + 1], pack_f32(relu_nan(x[2]), relu_nan(x[3])), s1);
           }
           if ((c + 1) % kPieces == 0) {
-            const int len = __shfl_sync(0xffffffffu, it.len, wg * kTok + tok);
-            if (key < len || (p.fill && key < p.num_keys))
+            if (key < len[tok] || (p.fill && key < p.num_keys))
               out[(size_t)tok * p.score_stride + key] =
-                  key < len && paged ? s0 + s1 : -CUDART_INF_F;
-            s0 = s1 = 0.0f;
+                  key < len[tok] && paged ? sum_f32(s0) + sum_f32(s1) : -CUDART_INF_F;
+            s0 = s1 = 0;
           }
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&ctl.acc_empty[b]));
-    }
-    if (!ok) break;
-    // Columns of the item that no token of the group sees.
-    const int c0 = it.tc * kIxKeys, c1 = min(it.t1 * kIxKeys, p.num_keys);
-    if (p.fill && c0 < c1) {
-      const bool vec = ((reinterpret_cast<uintptr_t>(p.scores) & 15) | (p.score_stride & 3)) == 0;
-      for (int t = 0; t < it.g.live; ++t) {
-        float* o = p.scores + (size_t)(it.g.tok0 + t) * p.score_stride;
-        if (vec) {
-          const float4 none = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-          for (int c = c0 + 4 * tid; c + 4 <= c1; c += 1024) *reinterpret_cast<float4*>(o + c) = none;
-          if (tid < (c1 & 3)) o[(c1 & ~3) + tid] = -CUDART_INF_F;
-        } else {
-          for (int c = c0 + tid; c < c1; c += 256) o[c] = -CUDART_INF_F;
-        }
-      }
+      if (lane == 0) arrive_remote(empty0 + 8u * (uint32_t)b);
     }
   }
 }
 
-template <bool kBf16, int kHp>
-__global__ void __launch_bounds__(kIxThreads, 1)
+// Items, their queries and weights, and the fill.
+template <int kChunks, int kHp>
+__device__ __forceinline__ void ix_items(const IxArgs& a, IxCtl& ctl, uint32_t sQ, int count,
+                                         int pair, int pairs, const CUtensorMap* tm_q, int rank,
+                                         int lane) {
+  const SasIndexParams& p = a.p;
+  const uint32_t full0 = peer_addr(smem_addr(&ctl.q_full[0]), 0);
+  const bool vec = ((reinterpret_cast<uintptr_t>(p.scores) & 15) | (p.score_stride & 3)) == 0;
+  int m = 0;
+  for (int i = 0; i < count; ++i) {
+    int t1;
+    const IxInfo r = ix_item(a, pair + i * pairs, lane, &t1);
+    const bool busy = r.tc > r.t0;
+    float w[kIxCols / 32];
+    if (busy) {
+#pragma unroll
+      for (int k = 0; k < kIxCols / 32; ++k) {
+        const int c = 32 * k + lane, t = c / kHp, h = c % kHp;
+        w[k] = t < r.live && h < p.num_heads
+                   ? __ldg(p.weights + (size_t)(p.first_token + r.tok0 + t) * p.num_heads + h)
+                   : 0.0f;
+      }
+    }
+    const int slot = i % kIxItems;
+    if (!ix_wait(ctl, &ctl.item_empty[slot], ((i / kIxItems) & 1) ^ 1, p.err, 68)) break;
+    IxInfo& o = ctl.items[slot];
+    if (lane == 0) {
+      o.tok0 = r.tok0;
+      o.live = r.live;
+      o.batch = r.batch;
+      o.most = r.most;
+      o.t0 = r.t0;
+      o.tc = r.tc;
+    }
+    if (lane < kIxTokens) o.len[lane] = r.len[0];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_addr(&ctl.item_full[slot]));
+    if (rank == 0 && r.t0 == 0 && p.lengths != nullptr && lane < r.live)
+      p.lengths[r.tok0 + lane] = r.len[0];
+    if (busy) {
+      const int qb = m & 1;
+      if (!ix_wait(ctl, &ctl.q_empty[qb], ((m >> 1) & 1) ^ 1, p.err, 72)) break;
+      // Each CTA holds the columns of half of the tokens.
+      const int half = (r.live + 1) >> 1;
+      const int mine = rank == 0 ? half : r.live - half;
+      const uint32_t bar = full0 + 8u * (uint32_t)qb;
+      if (lane == 0) arrive_tx_cluster(bar, (uint32_t)(mine * kChunks * kHp * 128), false);
+      __syncwarp();
+      if (lane < mine) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          tma_load_3d_pair(
+              sQ + (uint32_t)(qb * IxSmem<kChunks>::kQ + c * kIxQChunk + lane * kHp * 128), tm_q,
+              c * 64, 0, p.first_token + r.tok0 + rank * half + lane, bar);
+      }
+      if (!ix_wait(ctl, &ctl.w_empty, (m & 1) ^ 1, p.err, 78)) break;
+#pragma unroll
+      for (int k = 0; k < kIxCols / 32; ++k) ctl.w[32 * k + lane] = w[k];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&ctl.w_full));
+      ++m;
+    }
+    // Columns of the item that no token of the group sees: 32-lane pieces
+    // alternate between the CTAs.
+    const int c0 = r.tc * kIxTile, c1 = min(t1 * kIxTile, p.num_keys);
+    if (p.fill && c0 < c1) {
+      const float4 none = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+      const int first = 32 * rank + lane;
+      for (int t = 0; t < r.live; ++t) {
+        float* o2 = p.scores + (size_t)(r.tok0 + t) * p.score_stride;
+        if (vec) {
+          for (int c = c0 + 4 * first; c + 4 <= c1; c += 256) *reinterpret_cast<float4*>(o2 + c) = none;
+          if (first < (c1 & 3)) o2[(c1 & ~3) + first] = -CUDART_INF_F;
+        } else {
+          for (int c = c0 + first; c < c1; c += 64) o2[c] = -CUDART_INF_F;
+        }
+      }
+    }
+  }
+  // The leader's barriers count the queries of both CTAs.
+  if (rank == 0)
+    for (int k = max(0, m - 2); k < m; ++k) ix_settle(&ctl.q_full[k & 1], (uint32_t)(k >> 1) & 1);
+}
+
+template <int kChunks, int kHp>
+__device__ __forceinline__ void ix_issue(const IxArgs& a, IxCtl& ctl, uint32_t sQ, uint32_t sK,
+                                         uint32_t tmem, int count, int rank, int lane) {
+  using L = IxSmem<kChunks>;
+  const SasIndexParams& p = a.p;
+  int s = 0, ph = 0, b = 0, bph = 1;  // key stage, accumulator and the parities awaited
+  int m = 0;
+  const int steps = (p.head_dim + 15) / 16;
+  bool ok = true;
+  for (int i = 0; ok && i < count; ++i) {
+    const IxInfo* info = ix_next(ctl, i, p.err, 67);
+    if (info == nullptr) break;
+    const int t0 = info->t0, tc = info->tc;
+    const int cols = ((info->live + 1) & ~1) * kHp;
+    ix_done(ctl, i, lane);
+    if (rank != 0 || tc == t0) continue;
+    if (lane == 0) {
+      const int qb = m & 1;
+      const uint32_t idesc = a.idesc | (uint32_t)(cols >> 3) << 17;
+      const uint64_t dq = smem_desc(sQ + (uint32_t)(qb * L::kQ), 16, 1024);
+      ok = wait_bar(&ctl, &ctl.q_full[qb], (uint32_t)(m >> 1) & 1, p.err, 74);
+      for (int t = t0; ok && t < tc; ++t) {
+        ok = wait_bar(&ctl, &ctl.k_full[s], (uint32_t)ph, p.err, 75) &&
+             wait_bar(&ctl, &ctl.acc_empty[b], (uint32_t)bph, p.err, 76);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dk = smem_desc(sK + (uint32_t)(s * kChunks * kIxKChunk), 16, 1024);
+        const uint32_t acc = tmem + (uint32_t)(b * kIxCols);
+#pragma unroll
+        for (int k = 0; k < 4 * kChunks; ++k) {
+          const uint32_t in = (uint32_t)(k & 3) * 32u, ch = (uint32_t)(k >> 2);
+          if (k < steps)
+            mma2(acc, dk + ((in + ch * kIxKChunk) >> 4), dq + ((in + ch * kIxQChunk) >> 4), idesc,
+                 k > 0);
+        }
+        commit_both(smem_addr(&ctl.k_empty[s]));
+        commit_both(smem_addr(&ctl.acc_full[b]));
+        if (++s == L::kStages) {
+          s = 0;
+          ph ^= 1;
+        }
+        b ^= 1;
+        bph ^= b ^ 1;
+      }
+      commit_both(smem_addr(&ctl.q_empty[qb]));
+    }
+    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    ++m;
+  }
+  // Every MMA has read its operands before either CTA goes.
+  if (rank == 0 && lane == 0) {
+    commit_both(smem_addr(&ctl.drain));
+    ix_settle(&ctl.drain, 0u);
+  }
+}
+
+template <int kChunks, int kHp>
+__global__ void __launch_bounds__(kIxThreads, 1) __cluster_dims__(2, 1, 1)
     index_scores_kernel(const __grid_constant__ IxArgs a, const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ CUtensorMap tm_k) {
+  using L = IxSmem<kChunks>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const SasIndexParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int q_bytes = a.chunks * kIxQChunk, stage_bytes = a.chunks * kIxKChunk;
-  const uint32_t sQ = smem_addr(smem), sK = sQ + 2u * q_bytes;
-  IxCtl& ctl = *reinterpret_cast<IxCtl*>(smem + 2 * q_bytes + a.stages * stage_bytes);
+  const int rank = (int)cluster_rank();
+  const uint32_t sQ = smem_addr(smem), sK = sQ + 2u * L::kQ;
+  IxCtl& ctl = *reinterpret_cast<IxCtl*>(smem + L::kCtl);
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int items = a.groups * a.spans;
+  const int count = pair < items ? (items - pair + pairs - 1) / pairs : 0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&ctl.q_full[i]), 1);
+      mbar_init(smem_addr(&ctl.q_full[i]), 2);
       mbar_init(smem_addr(&ctl.q_empty[i]), 1);
-      mbar_init(smem_addr(&ctl.acc_full[i]), 2);
-      mbar_init(smem_addr(&ctl.acc_empty[i]), 8);
+      mbar_init(smem_addr(&ctl.acc_full[i]), 1);
+      mbar_init(smem_addr(&ctl.acc_empty[i]), 16);
     }
-    for (int i = 0; i < a.stages; ++i) {
-      mbar_init(smem_addr(&ctl.k_full[i]), 1);
+    for (int i = 0; i < kIxMaxStages; ++i) {
+      mbar_init(smem_addr(&ctl.k_full[i]), 2);
       mbar_init(smem_addr(&ctl.k_empty[i]), 1);
+      ctl.issued[i] = 0;
     }
+    for (int i = 0; i < kIxItems; ++i) {
+      mbar_init(smem_addr(&ctl.item_full[i]), 1);
+      mbar_init(smem_addr(&ctl.item_empty[i]), 11);  // warps 0, 1, 3 and the epilogue
+    }
+    for (int i = 0; i < kIxBits; ++i) mbar_init(smem_addr(&ctl.bits_full[i]), 1);
+    mbar_init(smem_addr(&ctl.w_full), 1);
+    mbar_init(smem_addr(&ctl.w_empty), 8);
     mbar_init(smem_addr(&ctl.drain), 1);
     ctl.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_addr(&ctl.tmem_base)),
                  "r"(2 * kIxCols)
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are initialised before any remote arrival
   tc_fence_after();
   const uint32_t tmem = ctl.tmem_base;
 
   if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kIxRegsEpi));
-    ix_epilogue<kHp>(a, ctl, tmem, items);
+    ix_epilogue<kHp>(a, ctl, tmem, count, rank);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIxRegsLoad));
-    if (warp == 0) {
-      // Keys.
-      int n = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; ok && item < items && !ctl.abort; item += gridDim.x) {
-        const IxItem it = ix_item(a, item, lane);
-        for (int t = it.t0; t < it.tc; ++t, ++n) {
-          const int s = n % a.stages;
-          const uint32_t stage = sK + (uint32_t)(s * stage_bytes);
-          const uint32_t bar = smem_addr(&ctl.k_full[s]);
-          int rows[4];
-          if (a.box_rows > 0) {
-            const int boxes = kIxKeys / a.box_rows;
-            rows[0] = lane < boxes
-                          ? ix_row(a, it.g.batch, t * kIxKeys + lane * a.box_rows, it.most)
-                          : a.no_row;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              rows[r] = ix_row(a, it.g.batch, t * kIxKeys + 4 * lane + r, it.most);
-          }
-          if (!__all_sync(0xffffffffu, wait_bar(&ctl, &ctl.k_empty[s],
-                                                (uint32_t)((n / a.stages) & 1) ^ 1, p.err, 70))) {
-            ok = false;
-            break;
-          }
-          uint32_t bits = 0;
-          if (a.box_rows > 0) {
-            const uint32_t mapped = __ballot_sync(0xffffffffu, rows[0] != a.no_row);
-            bits = (mapped >> (4 * lane / a.box_rows)) & 1 ? 15u : 0u;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) bits |= (rows[r] != a.no_row ? 1u : 0u) << r;
-          }
-          ctl.bits[n % kIxBits][lane] = (uint8_t)bits;
-          __syncwarp();
-          if (lane == 0) mbar_expect_tx(bar, (uint32_t)stage_bytes);
-          __syncwarp();
-          for (int c = 0; c < a.chunks; ++c) {
-            const uint32_t dst = stage + (uint32_t)(c * kIxKChunk);
-            if (a.box_rows == 0)
-              tma_gather4(dst + (uint32_t)lane * 512u, &tm_k, c * 64, rows[0], rows[1], rows[2],
-                          rows[3], bar);
-            else if (lane < kIxKeys / a.box_rows)
-              tma_load_2d(dst + (uint32_t)(lane * a.box_rows) * 128u, &tm_k, c * 64, rows[0], bar);
-          }
-        }
-      }
-      // Nothing may land after the block has gone: the last loads of each stage.
-      for (int k = max(0, n - a.stages); k < n; ++k)
-        ix_settle(&ctl.k_full[k % a.stages], (uint32_t)((k / a.stages) & 1));
-    } else if (warp == 1) {
-      // MMA.
-      int n = 0, m = 0;
-      bool ok = true;
-      const int steps = (p.head_dim + 15) / 16;
-      for (int item = blockIdx.x; ok && item < items && !ctl.abort; item += gridDim.x) {
-        const IxItem it = ix_item(a, item, lane);
-        if (it.tc == it.t0) continue;
-        if (lane == 0) {
-          const int qb = m & 1;
-          const uint32_t idesc = instr_desc(kIxKeys, it.g.live * kHp, kBf16, false, false);
-          const uint64_t dq = smem_desc(sQ + (uint32_t)(qb * q_bytes), 16, 1024);
-          ok = wait_bar(&ctl, &ctl.q_full[qb], (uint32_t)(m >> 1) & 1, p.err, 74);
-          for (int t = it.t0; ok && t < it.tc; ++t, ++n) {
-            const int s = n % a.stages, b = n & 1;
-            ok = wait_bar(&ctl, &ctl.k_full[s], (uint32_t)((n / a.stages) & 1), p.err, 75) &&
-                 wait_bar(&ctl, &ctl.acc_empty[b], (uint32_t)((n >> 1) & 1) ^ 1, p.err, 76);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t dk = smem_desc(sK + (uint32_t)(s * stage_bytes), 16, 1024);
-            for (int k = 0; k < steps; ++k) {
-              const uint32_t in = (uint32_t)(k & 3) * 32u;
-              ix_mma(tmem + (uint32_t)(b * kIxCols), dk + ((in + (uint32_t)(k >> 2) * kIxKChunk) >> 4),
-                     dq + ((in + (uint32_t)(k >> 2) * kIxQChunk) >> 4), idesc, k > 0);
-            }
-            tc_commit(smem_addr(&ctl.k_empty[s]));
-            mbar_arrive(smem_addr(&ctl.acc_full[b]));
-            tc_commit(smem_addr(&ctl.acc_full[b]));
-          }
-          tc_commit(smem_addr(&ctl.q_empty[qb]));
-        }
-        n = __shfl_sync(0xffffffffu, n, 0);
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        ++m;
-      }
-      if (lane == 0) {  // every MMA has read its operands before the block goes
-        tc_commit(smem_addr(&ctl.drain));
-        ix_settle(&ctl.drain, 0u);
-      }
-    } else if (warp == 2) {
-      // Queries.
-      int m = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; ok && item < items && !ctl.abort; item += gridDim.x) {
-        const IxItem it = ix_item(a, item, lane);
-        if (it.tc == it.t0) continue;
-        const int qb = m & 1;
-        if (!__all_sync(0xffffffffu, wait_bar(&ctl, &ctl.q_empty[qb], (uint32_t)((m >> 1) & 1) ^ 1,
-                                              p.err, 72))) {
-          ok = false;
-          break;
-        }
-        const uint32_t bar = smem_addr(&ctl.q_full[qb]);
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)(it.g.live * a.chunks * kHp * 128));
-        __syncwarp();
-        for (int i = lane; i < it.g.live * a.chunks; i += 32) {
-          const int c = i / it.g.live, t = i - c * it.g.live;
-          tma_load_3d(sQ + (uint32_t)(qb * q_bytes + c * kIxQChunk + t * kHp * 128), &tm_q, c * 64, 0,
-                      p.first_token + it.g.tok0 + t, bar);
-        }
-        ++m;
-      }
-      for (int k = max(0, m - 2); k < m; ++k)
-        ix_settle(&ctl.q_full[k & 1], (uint32_t)(k >> 1) & 1);
-    }
+    if (warp == 1)
+      ix_issue<kChunks, kHp>(a, ctl, sQ, sK, tmem, count, rank, lane);
+    else if (warp == 2)
+      ix_items<kChunks, kHp>(a, ctl, sQ, count, pair, pairs, &tm_q, rank, lane);
+    else
+      ix_keys<kChunks>(a, ctl, sK, count, &tm_k, warp == 3, rank, lane);
   }
 
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();
+  // Nothing may land after the pair has gone: loads that no MMA waited for
+  // after an abort complete on the leader's barriers.
+  if (rank == 0 && threadIdx.x == 0)
+    for (int i = 0; i < L::kStages; ++i)
+      if (ctl.issued[i] != 0) ix_settle(&ctl.k_full[i], ctl.issued[i] - 1u);
+  __syncthreads();
+  cluster_sync_all();
   if (warp == 2) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(2 * kIxCols)
                  : "memory");
   }
@@ -490,14 +679,14 @@ bool ix_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t mid, uint6
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool kBf16, int kHp>
+template <int kChunks, int kHp>
 int ix_launch(const IxArgs& a, int grid, const CUtensorMap& q, const CUtensorMap& k,
               cudaStream_t stream) {
-  // Per device: set on every call (a host call of well under a microsecond).
-  if (cudaFuncSetAttribute(index_scores_kernel<kBf16, kHp>,
+  // Per device, so set on every call (well under a microsecond).
+  if (cudaFuncSetAttribute(index_scores_kernel<kChunks, kHp>,
                            cudaFuncAttributeMaxDynamicSharedMemorySize, kIxSmem) != cudaSuccess)
     return SAS_ERR_CUDA;
-  index_scores_kernel<kBf16, kHp><<<grid, kIxThreads, kIxSmem, stream>>>(a, q, k);
+  index_scores_kernel<kChunks, kHp><<<grid, kIxThreads, kIxSmem, stream>>>(a, q, k);
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
 
@@ -533,50 +722,54 @@ extern "C" int sas_index_scores(const SasIndexParams* params, void* stream_ptr) 
 
   IxArgs a{};
   a.p = p;
-  a.hp = p.num_heads <= 16 ? 16 : p.num_heads <= 32 ? 32 : p.num_heads <= 64 ? 64 : 128;
-  a.tq = kIxCols / a.hp;
-  const int64_t groups =
-      ((int64_t)p.num_tokens + ((int64_t)p.batch + 1) * (a.tq - 1)) / a.tq;
-  a.tiles = (p.num_keys + kIxKeys - 1) / kIxKeys;
-  // Spans: short enough for about 16 items a block, so that blocks end
+  const int hp = p.num_heads <= 16 ? 16 : p.num_heads <= 32 ? 32 : p.num_heads <= 64 ? 64 : 128;
+  const int tq = kIxCols / hp;
+  while ((1 << a.tq_shift) < tq) ++a.tq_shift;
+  const int64_t groups = ((int64_t)p.num_tokens + ((int64_t)p.batch + 1) * (tq - 1)) / tq;
+  a.tiles = (p.num_keys + kIxTile - 1) / kIxTile;
+  // Spans: short enough for about 16 items a pair, so that pairs end
   // together; whole rows where the groups alone are that many.
+  const int pairs = sms / 2;
   const int64_t total = groups * (a.tiles > 0 ? a.tiles : 1);
-  const int64_t span = (total + 16 * sms - 1) / (16 * sms);
+  const int64_t span = (total + 16 * pairs - 1) / (16 * pairs);
   a.span_tiles = (int)(span < 1 ? 1 : span > a.tiles ? (a.tiles > 0 ? a.tiles : 1) : span);
   a.spans = a.tiles > 0 ? (a.tiles + a.span_tiles - 1) / a.span_tiles : 1;
   if (groups * a.spans > INT32_MAX - 4096) return SAS_ERR_UNSUPPORTED;
   a.groups = (int)groups;
   a.no_row = p.num_blocks * p.block_size;
-  a.chunks = p.head_dim > 64 ? 2 : 1;
-  a.stages = (kIxSmem - (int)sizeof(IxCtl) - 2 * a.chunks * kIxQChunk) / (a.chunks * kIxKChunk);
-  if (a.stages > kIxMaxStages) a.stages = kIxMaxStages;
+  a.idesc = instr_desc(kIxTile, 0, p.dtype == SAS_DTYPE_BF16, false, false);
   // Box of key rows: the largest power of two up to 128 that divides the page
   // (a box then never leaves its page); pages that 8 does not divide are
   // gathered row by row.
   int box = 128;
   while (box >= 8 && p.block_size % box != 0) box >>= 1;
-  a.box_rows = box >= 8 ? box : 0;
+  if (box >= 8)
+    while ((1 << a.box_shift) < box) ++a.box_shift;
+  else
+    box = 1;
 
   alignas(64) CUtensorMap tm_q, tm_k;
   const uint64_t D = (uint64_t)p.head_dim, H = (uint64_t)p.num_heads, T = (uint64_t)p.total_tokens;
-  if (!ix_map(&tm_q, p.q, D, H, T, (uint32_t)a.hp, true)) return SAS_ERR_CUDA;
+  if (!ix_map(&tm_q, p.q, D, H, T, (uint32_t)hp, true)) return SAS_ERR_CUDA;
   if (a.no_row > 0) {
-    if (!ix_map(&tm_k, p.key_pool, D, (uint64_t)a.no_row, 1, a.box_rows > 0 ? a.box_rows : 1, false))
+    if (!ix_map(&tm_k, p.key_pool, D, (uint64_t)a.no_row, 1, (uint32_t)box, false))
       return SAS_ERR_CUDA;
   } else {
     // An empty pool: every page is unmapped, and the row past it has to read
     // as zeros, as the row past the queries does.
     if (T * H > INT32_MAX - 1) return SAS_ERR_UNSUPPORTED;
     a.no_row = (int)(T * H);
-    if (!ix_map(&tm_k, p.q, D, T * H, 1, a.box_rows > 0 ? a.box_rows : 1, false))
+    if (!ix_map(&tm_k, p.q, D, T * H, 1, (uint32_t)box, false))
       return SAS_ERR_CUDA;
   }
   const int64_t items = (int64_t)a.groups * a.spans;
-  const int grid = (int)(items < sms ? items : sms);
+  const int grid = 2 * (int)(items < pairs ? items : pairs);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-#define SAS_IX(HP)                                                                      \
-  (p.dtype == SAS_DTYPE_BF16 ? ix_launch<true, HP>(a, grid, tm_q, tm_k, stream)         \
-                             : ix_launch<false, HP>(a, grid, tm_q, tm_k, stream))
-  return a.hp == 16 ? SAS_IX(16) : a.hp == 32 ? SAS_IX(32) : a.hp == 64 ? SAS_IX(64) : SAS_IX(128);
+#define SAS_IX(C)                                                       \
+  (hp == 16   ? ix_launch<C, 16>(a, grid, tm_q, tm_k, stream)           \
+   : hp == 32 ? ix_launch<C, 32>(a, grid, tm_q, tm_k, stream)           \
+   : hp == 64 ? ix_launch<C, 64>(a, grid, tm_q, tm_k, stream)           \
+              : ix_launch<C, 128>(a, grid, tm_q, tm_k, stream))
+  return p.head_dim > 64 ? SAS_IX(2) : SAS_IX(1);
 #undef SAS_IX
 }
