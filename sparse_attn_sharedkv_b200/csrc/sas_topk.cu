@@ -4,19 +4,41 @@
 // (golden.py:28-66 stops at the first -1).  A score of -inf is never
 // selected; NaN ranks above +inf and -0 equals +0.
 //
-// A score becomes an unsigned key of the same order.  One block per row finds
-// the K-th largest key by four passes of 8 bits, then writes the positions
-// above it and the first ties by a scan over the row.
+// A score becomes an unsigned key of the same order.  A row is read once and
+// stays in the registers of a block, 16 keys a thread, or of a cluster of up
+// to 8 blocks that exchange a few values through distributed shared memory:
+//
+//   1. the least and the greatest finite key, and how many keys can be
+//      selected (no more than K: all of them are);
+//   2. a histogram of 1024 bins between the two, linear in the scores, so
+//      that near-normal scores spread over it (a bin then holds a few, and
+//      the shared-memory atomics seldom meet); the bin in which the K-th
+//      largest lies: keys in higher bins are selected;
+//   3. while that bin holds more than 128 keys: the same between the least and
+//      the greatest key of the bin, linear in the keys, which divides their
+//      range by at least 512 and so ends after at most four rounds;
+//   4. the keys of the last bin are listed and ranked by (key, position); the
+//      last one taken is the threshold.  Equal keys that fill a bin of more
+//      than 128 are taken by a count over the positions instead;
+//   5. the selected positions are counted and written.
+//
+// Thread t of a block holds the positions begin + 16 T's worth at a stride of
+// T: loads are coalesced for any row alignment, a ballot a round counts the
+// selected lanes, and these write neighbouring words.
 
 #include <cuda_runtime.h>
+#include <math_constants.h>
 #include <stdint.h>
 
 #include "sas.h"
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kBins = 1024;
+constexpr int kList = 128;                 // keys ranked directly
+constexpr int kPer = 16;                   // keys of a thread
 constexpr uint32_t kNegInf = 0x007fffffu;  // key of -inf
+constexpr uint32_t kPosInf = 0xff800000u;  // key of +inf
 
 __device__ __forceinline__ uint32_t key_of(float x) {
   if (x != x) return 0xffffffffu;
@@ -24,26 +46,386 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kThreads)
-    topk_kernel(const float* __restrict__ scores, int64_t stride, const int32_t* __restrict__ lengths,
-                int n_cols, int K, int32_t* __restrict__ out) {
+__device__ __forceinline__ float score_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
+}
+
+// Address of `p` (own shared memory) in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_smem(const void* p, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(r)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t peer_load(const void* p, int rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_smem(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void peer_store(void* p, int rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_smem(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t peer_add(void* p, int rank, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;"
+               : "=r"(old)
+               : "r"(peer_smem(p, rank)), "r"(v)
+               : "memory");
+  return old;
+}
+
+template <int C>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (C == 1)
+    __syncthreads();
+  else
+    asm volatile(
+        "barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+            : "memory");
+}
+
+// Shared memory of a block.
+template <int T, int C>
+struct TopkShared {
+  alignas(16) uint32_t hist[kBins];  // from the top bin down
+  alignas(16) uint32_t wtot[kPer * (T / 32)];
+  uint32_t wmin[T / 32], wmax[T / 32], wcnt[T / 32], wsum[T / 32];
+  uint32_t rmin[C], rmax[C], rcnt[C], rtot[C];  // one entry per block of the cluster
+  uint32_t bin, above, inside;                  // found in the histogram, bin from the top
+  uint32_t listed;
+  uint32_t list_key[kList], list_pos[kList];  // of the cluster, in block 0
+  uint32_t key[kList], pos[kList];            // own copy
+  uint32_t thr_key, thr_pos;
+};
+
+// Least and greatest of the keys (kmin, kmax) and the sum of n over the row's
+// threads.
+template <int T, int C>
+__device__ __forceinline__ void row_reduce(TopkShared<T, C>& s, int rank, uint32_t& kmin,
+                                           uint32_t& kmax, uint32_t& n) {
+  constexpr int W = T / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  kmin = __reduce_min_sync(0xffffffffu, kmin);
+  kmax = __reduce_max_sync(0xffffffffu, kmax);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (lane == 0) {
+    s.wmin[warp] = kmin;
+    s.wmax[warp] = kmax;
+    s.wcnt[warp] = n;
+  }
+  __syncthreads();
+  kmin = __reduce_min_sync(0xffffffffu, lane < W ? s.wmin[lane] : 0xffffffffu);
+  kmax = __reduce_max_sync(0xffffffffu, lane < W ? s.wmax[lane] : 0u);
+  n = __reduce_add_sync(0xffffffffu, lane < W ? s.wcnt[lane] : 0u);
+  if constexpr (C > 1) {
+    if (warp == 0 && lane < C) {
+      peer_store(&s.rmin[rank], lane, kmin);
+      peer_store(&s.rmax[rank], lane, kmax);
+      peer_store(&s.rcnt[rank], lane, n);
+    }
+    row_sync<C>();
+    kmin = __reduce_min_sync(0xffffffffu, lane < C ? s.rmin[lane] : 0xffffffffu);
+    kmax = __reduce_max_sync(0xffffffffu, lane < C ? s.rmax[lane] : 0u);
+    n = __reduce_add_sync(0xffffffffu, lane < C ? s.rcnt[lane] : 0u);
+  }
+}
+
+// The bin of the histograms (of all the row's blocks) in which the need-th
+// largest lies: into s.bin, with the count above it and the one inside.
+// Starts and ends with a barrier of the row / the block.
+template <int T, int C>
+__device__ __forceinline__ void find_bin(TopkShared<T, C>& s, uint32_t need) {
+  constexpr int W = T / 32, kOwn = kBins / T;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  row_sync<C>();
+  uint32_t h[kOwn], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const int b = tid * kOwn + i;
+    h[i] = 0;
+    if constexpr (C == 1) {
+      h[i] = s.hist[b];
+    } else {
+#pragma unroll
+      for (int r = 0; r < C; ++r) h[i] += peer_load(&s.hist[b], r);
+    }
+    sum += h[i];
+  }
+  uint32_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) s.wsum[warp] = incl;
+  __syncthreads();
+  uint32_t before = __reduce_add_sync(0xffffffffu, lane < W && lane < warp ? s.wsum[lane] : 0u);
+  before += incl - sum;
+  if (before < need && need <= before + sum) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      if (before < need && need <= before + h[i]) {
+        s.bin = (uint32_t)(tid * kOwn + i);
+        s.above = before;
+        s.inside = h[i];
+      }
+      before += h[i];
+    }
+  }
+  __syncthreads();
+}
+
+// Count, over the row's positions, of the flags (bit i: the thread's key of
+// round i) before each of the thread's keys: at[i] for round i.  Returns the
+// block's total and, in *block_base, the count in the blocks before it.
+template <int T, int C>
+__device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, uint32_t flags,
+                                                 uint32_t (&at)[kPer], uint32_t* block_base) {
+  constexpr int W = T / 32, kChunk = W / 2;  // kPer * W counts: kChunk of them a lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t below = (1u << lane) - 1u;
+  uint32_t own = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t m = __ballot_sync(0xffffffffu, flags >> i & 1);
+    at[i] = __popc(m & below);
+    if (lane == i) own = __popc(m);
+  }
+  __syncthreads();
+  if (lane < kPer) s.wtot[lane * W + warp] = own;
+  __syncthreads();
+  // Lane l: counts l kChunk .. of the rounds in order, their sum and the part
+  // before this warp's inside the chunk.
+  uint32_t sum = 0, part = 0;
+#pragma unroll
+  for (int k = 0; k < kChunk; ++k) {
+    const uint32_t v = s.wtot[lane * kChunk + k];
+    part += k < warp % kChunk ? v : 0u;
+    sum += v;
+  }
+  uint32_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  const uint32_t start = incl - sum + part;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    at[i] += __shfl_sync(0xffffffffu, start, 2 * i + (warp >= kChunk ? 1 : 0));
+  const uint32_t total = __shfl_sync(0xffffffffu, incl, 31);
+  *block_base = 0;
+  if constexpr (C > 1) {
+    if (warp == 0 && lane < C) peer_store(&s.rtot[rank], lane, total);
+    row_sync<C>();
+    *block_base = __reduce_add_sync(0xffffffffu, lane < rank ? s.rtot[lane] : 0u);
+  }
+  return total;
+}
+
+template <int T, int C>
+__global__ void __launch_bounds__(T) __cluster_dims__(C, 1, 1)
+    topk_kernel(const float* __restrict__ scores, int64_t stride,
+                const int32_t* __restrict__ lengths, int n_cols, int K,
+                int32_t* __restrict__ out) {
+  __shared__ TopkShared<T, C> s;
+  const int tid = threadIdx.x;
+  const int rank = C == 1 ? 0 : (int)(blockIdx.x % C);
+  const int64_t row = blockIdx.x / C;
+  const float* x = scores + row * stride;
+  int32_t* o = out + row * K;
+  int n = n_cols;
+  if (lengths != nullptr) n = max(0, min(n, __ldg(lengths + row)));
+  // The block's part of the row.
+  const int part = (n + C - 1) / C;
+  const int begin = min(n, rank * part), end = min(n, begin + part);
+
+  uint32_t key[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int p = begin + i * T + tid;
+    key[i] = p < end ? key_of(__ldg(x + p)) : 0u;
+  }
+  for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+  if (tid == 0) s.listed = 0;
+
+  uint32_t kmin = 0xffffffffu, kmax = 0, able = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (key[i] > kNegInf) {
+      ++able;
+      if (key[i] < kPosInf) {
+        kmin = min(kmin, key[i]);
+        kmax = max(kmax, key[i]);
+      }
+    }
+  }
+  row_reduce<T, C>(s, rank, kmin, kmax, able);
+
+  uint32_t sel = 0;  // bit i: key[i] is selected
+  if (able <= (uint32_t)K) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sel |= (key[i] > kNegInf ? 1u : 0u) << i;
+  } else {
+    // Linear in the scores; a range whose scale is not finite (it overflows,
+    // is subnormal or a single value) puts every finite score into the last bin.
+    const float low = score_of(kmin);
+    float scale = kmin <= kmax ? __fdividef(kBins - 0.5f, score_of(kmax) - low) : 0.0f;
+    if (!(scale < CUDART_INF_F)) scale = 0.0f;
+    auto bin_of = [&](uint32_t k) {
+      if (k >= kPosInf) return 0;
+      // An infinite difference times a scale of zero is NaN, which max takes to 0.
+      return kBins - 1 - (int)fminf(fmaxf((score_of(k) - low) * scale, 0.0f), (float)(kBins - 1));
+    };
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (key[i] > kNegInf) atomicAdd(&s.hist[bin_of(key[i])], 1u);
+    uint32_t need = (uint32_t)K;
+    find_bin<T, C>(s, need);
+    uint32_t cand = 0;
+    int bin = (int)s.bin;
+    need -= s.above;
+    uint32_t inside = s.inside;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (key[i] > kNegInf) {
+        const int b = bin_of(key[i]);
+        sel |= (b < bin ? 1u : 0u) << i;
+        cand |= (b == bin ? 1u : 0u) << i;
+      }
+    }
+    bool equal = false;
+    while (inside > need && inside > kList) {
+      kmin = 0xffffffffu;
+      kmax = 0;
+      uint32_t none = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (cand >> i & 1) {
+          kmin = min(kmin, key[i]);
+          kmax = max(kmax, key[i]);
+        }
+      }
+      row_reduce<T, C>(s, rank, kmin, kmax, none);
+      if (kmin == kmax) {
+        equal = true;
+        break;
+      }
+      // Every block of the row has read the histograms: its last barrier was
+      // behind them.
+      for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+      __syncthreads();
+      const int shift = max(0, 22 - __clz(kmax - kmin));  // range >> shift below 1024
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (cand >> i & 1) atomicAdd(&s.hist[kBins - 1 - (int)((key[i] - kmin) >> shift)], 1u);
+      find_bin<T, C>(s, need);
+      bin = (int)s.bin;
+      need -= s.above;
+      inside = s.inside;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (cand >> i & 1) {
+          const int b = kBins - 1 - (int)((key[i] - kmin) >> shift);
+          sel |= (b < bin ? 1u : 0u) << i;
+          if (b != bin) cand &= ~(1u << i);
+        }
+      }
+    }
+    if (inside == need) {
+      sel |= cand;
+    } else if (equal) {
+      // The first `need` of the equal keys by position.
+      uint32_t at[kPer], base;
+      count_before<T, C>(s, rank, cand, at, &base);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (cand >> i & 1) sel |= (base + at[i] < need ? 1u : 0u) << i;
+      row_sync<C>();  // before the counts are written again
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (cand >> i & 1) {
+          const uint32_t p = (uint32_t)(begin + i * T + tid);
+          if constexpr (C == 1) {
+            const uint32_t l = atomicAdd(&s.listed, 1u);
+            s.key[l] = key[i];
+            s.pos[l] = p;
+          } else {
+            const uint32_t l = peer_add(&s.listed, 0, 1u);
+            peer_store(&s.list_key[l], 0, key[i]);
+            peer_store(&s.list_pos[l], 0, p);
+          }
+        }
+      }
+      row_sync<C>();
+      if constexpr (C > 1) {
+        if (tid < (int)inside) {
+          s.key[tid] = peer_load(&s.list_key[tid], 0);
+          s.pos[tid] = peer_load(&s.list_pos[tid], 0);
+        }
+        __syncthreads();
+      }
+      if (tid < (int)inside) {
+        const uint32_t k = s.key[tid], p = s.pos[tid];
+        uint32_t r = 0;
+        for (int j = 0; j < (int)inside; ++j)
+          r += s.key[j] > k || (s.key[j] == k && s.pos[j] < p) ? 1u : 0u;
+        if (r + 1 == need) {
+          s.thr_key = k;
+          s.thr_pos = p;
+        }
+      }
+      __syncthreads();
+      const uint32_t tk = s.thr_key, tp = s.thr_pos;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (cand >> i & 1) {
+          const uint32_t p = (uint32_t)(begin + i * T + tid);
+          sel |= (key[i] > tk || (key[i] == tk && p <= tp) ? 1u : 0u) << i;
+        }
+      }
+    }
+  }
+
+  uint32_t at[kPer], base;
+  count_before<T, C>(s, rank, sel, at, &base);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (sel >> i & 1) o[base + at[i]] = begin + i * T + tid;
+  const uint32_t filled = min(able, (uint32_t)K);
+  for (uint32_t i = filled + rank * T + tid; i < (uint32_t)K; i += C * T) o[i] = -1;
+  if constexpr (C > 1) row_sync<C>();  // no block leaves while another reads its shared memory
+}
+
+// Rows longer than a cluster holds: one block per row, the K-th largest key by
+// four passes of 8 bits over the row, then the positions above it and the
+// first ties by a scan over the row.
+constexpr int kLongThreads = 1024;
+
+__global__ void __launch_bounds__(kLongThreads)
+    topk_long_kernel(const float* __restrict__ scores, int64_t stride,
+                     const int32_t* __restrict__ lengths, int n_cols, int K,
+                     int32_t* __restrict__ out) {
   __shared__ uint32_t hist[256];
   __shared__ uint32_t sh_prefix, sh_need, sh_total;
-  __shared__ int warp_gt[kThreads / 32], warp_eq[kThreads / 32];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float* x = scores + (size_t)row * stride;
-  int32_t* o = out + (size_t)row * K;
+  __shared__ int warp_gt[kLongThreads / 32], warp_eq[kLongThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x;
+  const float* x = scores + row * stride;
+  int32_t* o = out + row * K;
   int n = n_cols;
   if (lengths != nullptr) n = max(0, min(n, lengths[row]));
   // Digits of the threshold key, from the top.
   uint32_t prefix = 0, need = K;
   bool all = false;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+    for (int i = tid; i < 256; i += kLongThreads) hist[i] = 0;
     if (tid == 0) sh_total = 0;
     __syncthreads();
     const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int i = tid; i < n; i += kThreads) {
+    for (int64_t i = tid; i < n; i += kLongThreads) {
       const uint32_t k = key_of(x[i]);
       if (k > kNegInf && (k & high) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
     }
@@ -69,8 +451,8 @@ __global__ void __launch_bounds__(kThreads)
     __syncthreads();
   }
   int done = 0, ties = 0;
-  for (int i0 = 0; i0 < n; i0 += kThreads) {
-    const int i = i0 + tid;
+  for (int64_t i0 = 0; i0 < n; i0 += kLongThreads) {
+    const int64_t i = i0 + tid;
     const uint32_t k = i < n ? key_of(x[i]) : 0u;
     const bool gt = all ? k > kNegInf : k > prefix;
     const bool eq = !all && i < n && k == prefix;
@@ -80,26 +462,20 @@ __global__ void __launch_bounds__(kThreads)
       warp_eq[warp] = __popc(me);
     }
     __syncthreads();
-    int g = done, e = ties;
-    for (int w = 0; w < warp; ++w) {
-      g += warp_gt[w];
-      e += warp_eq[w];
-    }
+    const int vg = warp_gt[lane], ve = warp_eq[lane];
     const uint32_t below = (1u << lane) - 1u;
-    e += __popc(me & below);
-    g += __popc(mg & below);
+    const int g = done + __reduce_add_sync(0xffffffffu, lane < warp ? vg : 0) + __popc(mg & below);
+    const int e = ties + __reduce_add_sync(0xffffffffu, lane < warp ? ve : 0) + __popc(me & below);
     // Position in the output: those above before it plus the ties taken.
     const int at = g + min(e, (int)need);
-    if (gt) o[all ? g : at] = i;
-    if (eq && e < (int)need) o[at] = i;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      done += warp_gt[w];
-      ties += warp_eq[w];
-    }
+    if (gt) o[all ? g : at] = (int32_t)i;
+    if (eq && e < (int)need) o[at] = (int32_t)i;
+    done += __reduce_add_sync(0xffffffffu, vg);
+    ties += __reduce_add_sync(0xffffffffu, ve);
     __syncthreads();
   }
   const int filled = all ? done : K;
-  for (int i = filled + tid; i < K; i += kThreads) o[i] = -1;
+  for (int i = filled + tid; i < K; i += kLongThreads) o[i] = -1;
 }
 
 }  // namespace
@@ -110,7 +486,23 @@ extern "C" int sas_topk_select(const float* scores, int64_t score_stride, const 
   if (rows < 0 || num_keys < 0 || topk < 1 || score_stride < num_keys) return SAS_ERR_INVALID;
   if (rows == 0) return SAS_OK;
   if (!indices || (num_keys > 0 && !scores)) return SAS_ERR_INVALID;
-  topk_kernel<<<rows, kThreads, 0, reinterpret_cast<cudaStream_t>(stream_ptr)>>>(
-      scores, score_stride, lengths, num_keys, topk, indices);
+  if (rows > INT32_MAX / 8) return SAS_ERR_UNSUPPORTED;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
+  // The smallest block whose registers hold the row, then clusters of blocks
+  // of 512 threads (8192 keys), then of 1024.
+#define SAS_TOPK(T, C)                                                                           \
+  topk_kernel<T, C><<<(unsigned)rows * C, T, 0, stream>>>(scores, score_stride, lengths, num_keys, \
+                                                          topk, indices)
+  if (num_keys <= kPer * 128) SAS_TOPK(128, 1);
+  else if (num_keys <= kPer * 256) SAS_TOPK(256, 1);
+  else if (num_keys <= kPer * 512) SAS_TOPK(512, 1);
+  else if (num_keys <= kPer * 512 * 2) SAS_TOPK(512, 2);
+  else if (num_keys <= kPer * 512 * 4) SAS_TOPK(512, 4);
+  else if (num_keys <= kPer * 512 * 8) SAS_TOPK(512, 8);
+  else if (num_keys <= kPer * 1024 * 8) SAS_TOPK(1024, 8);
+  else
+    topk_long_kernel<<<rows, kLongThreads, 0, stream>>>(scores, score_stride, lengths, num_keys,
+                                                        topk, indices);
+#undef SAS_TOPK
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
