@@ -4,27 +4,30 @@
 // (golden.py:28-66 stops at the first -1).  A score of -inf is never
 // selected; NaN ranks above +inf and -0 equals +0.
 //
-// A score becomes an unsigned key of the same order.  A row is read once and
-// stays in the registers of a block, 16 keys a thread, or of a cluster of up
-// to 8 blocks that exchange a few values through distributed shared memory:
+// A row is read once and stays in the registers of a block, 16 scores a
+// thread, or of a cluster of up to 8 blocks that exchange a few values through
+// distributed shared memory.  Rows of finite scores (the ordinary case):
 //
-//   1. the least and the greatest finite key, and how many keys can be
-//      selected (no more than K: all of them are);
-//   2. a histogram of 1024 bins between the two, linear in the scores, so
-//      that near-normal scores spread over it (a bin then holds a few, and
-//      the shared-memory atomics seldom meet); the bin in which the K-th
-//      largest lies: keys in higher bins are selected;
-//   3. while that bin holds more than 128 keys: the same between the least and
-//      the greatest key of the bin, linear in the keys, which divides their
-//      range by at least 512 and so ends after at most four rounds;
-//   4. the keys of the last bin are listed and ranked by (key, position); the
-//      last one taken is the threshold.  Equal keys that fill a bin of more
-//      than 128 are taken by a count over the positions instead;
-//   5. the selected positions are counted and written.
+//   1. the least and the greatest score; a row of at most K is all selected;
+//   2. a histogram of 1024 bins linear in the scores, over which near-normal
+//      scores spread (a bin then holds a few, and the shared-memory atomics
+//      seldom meet); the bin in which the K-th largest lies.  The bin is the
+//      low bits of a float near 2^23, so no conversion is needed;
+//   3. if that bin holds more than 128, once more inside of it;
+//   4. the scores of the last bin are listed and ranked by (score, position):
+//      the K-th is the threshold;
+//   5. the positions at or above the threshold are counted and written.
 //
-// Thread t of a block holds the positions begin + 16 T's worth at a stride of
-// T: loads are coalesced for any row alignment, a ballot a round counts the
-// selected lanes, and these write neighbouring words.
+// Any other row (infinities, NaN, a single value, more than 128 left after
+// step 3) is read again as unsigned keys of the same order: histograms linear
+// in the keys divide the range of the border keys by at least 512 a round
+// until 128 or a single key are left; equal keys are taken by a count over
+// their positions.
+//
+// Thread t of a block holds the positions at a stride of T: loads are
+// coalesced for any row alignment.  The flags of four rounds are four bytes of
+// a word, so one shuffle scan counts them, and the selected lanes of a round
+// write neighbouring words.
 
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -184,16 +187,26 @@ __device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, 
                                                  uint32_t (&at)[kPer], uint32_t* block_base) {
   constexpr int W = T / 32, kChunk = W / 2;  // kPer * W counts: kChunk of them a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t below = (1u << lane) - 1u;
-  uint32_t own = 0;
+  uint32_t incl4[kPer / 4];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const uint32_t m = __ballot_sync(0xffffffffu, flags >> i & 1);
-    at[i] = __popc(m & below);
-    if (lane == i) own = __popc(m);
+  for (int g = 0; g < kPer / 4; ++g) {
+    // Bits 0 .. 3 of the group into the low bits of four bytes.
+    const uint32_t own = ((flags >> (4 * g) & 15u) * 0x00204081u) & 0x01010101u;
+    uint32_t v = own;  // at most 32 in each byte
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    incl4[g] = v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) at[4 * g + k] = ((v - own) >> (8 * k)) & 255u;
   }
   __syncthreads();
-  if (lane < kPer) s.wtot[lane * W + warp] = own;
+  if (lane == 31) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s.wtot[i * W + warp] = (incl4[i / 4] >> (8 * (i % 4))) & 255u;
+  }
   __syncthreads();
   // Lane l: counts l kChunk .. of the rounds in order, their sum and the part
   // before this warp's inside the chunk.
@@ -224,23 +237,12 @@ __device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, 
   return total;
 }
 
+// Selection flags of any row, by keys.  Shared memory is in use up to here by
+// no thread of the row.
 template <int T, int C>
-__global__ void __launch_bounds__(T) __cluster_dims__(C, 1, 1)
-    topk_kernel(const float* __restrict__ scores, int64_t stride,
-                const int32_t* __restrict__ lengths, int n_cols, int K,
-                int32_t* __restrict__ out) {
-  __shared__ TopkShared<T, C> s;
+__device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float* x, int begin,
+                                                int end, int rank, int K, uint32_t* selectable) {
   const int tid = threadIdx.x;
-  const int rank = C == 1 ? 0 : (int)(blockIdx.x % C);
-  const int64_t row = blockIdx.x / C;
-  const float* x = scores + row * stride;
-  int32_t* o = out + row * K;
-  int n = n_cols;
-  if (lengths != nullptr) n = max(0, min(n, __ldg(lengths + row)));
-  // The block's part of the row.
-  const int part = (n + C - 1) / C;
-  const int begin = min(n, rank * part), end = min(n, begin + part);
-
   uint32_t key[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -248,7 +250,6 @@ __global__ void __launch_bounds__(T) __cluster_dims__(C, 1, 1)
     key[i] = p < end ? key_of(__ldg(x + p)) : 0u;
   }
   for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
-  if (tid == 0) s.listed = 0;
 
   uint32_t kmin = 0xffffffffu, kmax = 0, able = 0;
 #pragma unroll
@@ -387,6 +388,193 @@ __global__ void __launch_bounds__(T) __cluster_dims__(C, 1, 1)
         }
       }
     }
+  }
+
+  *selectable = able;
+  return sel;
+}
+
+// redux over the warp, NaN if any is.
+__device__ __forceinline__ float warp_min(float v) {
+  float r;
+  asm("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 1280 threads an SM where the block size allows: 48 registers a thread, which
+// hold the ordinary path without spills.
+template <int T, int C>
+__global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C, 1, 1)
+    topk_kernel(const float* __restrict__ scores, int64_t stride,
+                const int32_t* __restrict__ lengths, int n_cols, int K,
+                int32_t* __restrict__ out) {
+  constexpr int W = T / 32;
+  constexpr float kShift = 8388608.0f;         // 2^23: integers are its low bits
+  constexpr uint32_t kShiftBits = 0x4b000000u;
+  __shared__ TopkShared<T, C> s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = C == 1 ? 0 : (int)(blockIdx.x % C);
+  const int64_t row = blockIdx.x / C;
+  const float* x = scores + row * stride;
+  int32_t* o = out + row * K;
+  int n = n_cols;
+  if (lengths != nullptr) n = max(0, min(n, __ldg(lengths + row)));
+  if (n == 0) {  // the whole row's blocks alike
+    for (int i = rank * T + tid; i < K; i += C * T) o[i] = -1;
+    return;
+  }
+  // The block's part of the row; rounds in which the thread holds a score.
+  const int part = (n + C - 1) / C;
+  const int begin = min(n, rank * part), end = min(n, begin + part);
+  const int rounds = (end - begin - tid + T - 1) / T;
+
+  // Empty places hold the row's first score, which changes no extremum.
+  const float first = __ldg(x);
+  float v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) v[i] = i < rounds ? __ldg(x + begin + i * T + tid) : first;
+  for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+  if (tid == 0) s.listed = 0;
+
+  float low = v[0], high = v[0];
+#pragma unroll
+  for (int i = 1; i < kPer; ++i) {
+    low = min_nan(low, v[i]);
+    high = max_nan(high, v[i]);
+  }
+  low = warp_min(low);
+  high = warp_max(high);
+  if (lane == 0) {
+    s.wmin[warp] = __float_as_uint(low);
+    s.wmax[warp] = __float_as_uint(high);
+  }
+  __syncthreads();
+  low = warp_min(__uint_as_float(s.wmin[lane % W]));
+  high = warp_max(__uint_as_float(s.wmax[lane % W]));
+  if constexpr (C > 1) {
+    if (warp == 0 && lane < C) {
+      peer_store(&s.rmin[rank], lane, __float_as_uint(low));
+      peer_store(&s.rmax[rank], lane, __float_as_uint(high));
+    }
+    row_sync<C>();
+    low = warp_min(__uint_as_float(s.rmin[lane % C]));
+    high = warp_max(__uint_as_float(s.rmax[lane % C]));
+  }
+
+  uint32_t sel = 0, able = (uint32_t)n;
+  const float scale = __fdividef((float)(kBins - 2), high - low);
+  bool general = false;
+  if (low > -CUDART_INF_F && n <= K) {
+    // Every score is selected.
+    for (int i = begin + tid; i < end; i += T) o[i] = i;
+    for (int i = n + rank * T + tid; i < K; i += C * T) o[i] = -1;
+    return;
+  }
+  if (low > -CUDART_INF_F && high < CUDART_INF_F && scale > 0.0f && scale < CUDART_INF_F) {
+    uint32_t need = (uint32_t)K;
+    // 2^23 plus the bin of a score, rounded: non-decreasing in the score.
+    auto place = [&](float a) { return fmaf(a - low, scale, kShift); };
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i < rounds)
+        atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place(v[i]))], 1u);
+    find_bin<T, C>(s, need);
+    const float bin = kShift + (float)(kBins - 1 - (int)s.bin);
+    need -= s.above;
+    uint32_t inside = s.inside;
+    // A second histogram over the bin's scores: bin - 0.5 .. bin + 0.5 of the
+    // first, cut to its 1024 bins, is non-decreasing in the score again.
+    const float edge = bin - kShift - 0.5f;
+    auto place2 = [&](float a) {
+      const float u = fmaf(a - low, scale, -edge);
+      return fminf(fmaxf(u * (float)kBins, 0.0f), (float)(kBins - 1)) + kShift;
+    };
+    float bin2 = 0.0f;
+    const bool twice = inside > need && inside > kList;
+    if (twice) {
+      row_sync<C>();  // every block has read the first histogram
+      for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < rounds && place(v[i]) == bin)
+          atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place2(v[i]))], 1u);
+      find_bin<T, C>(s, need);
+      bin2 = kShift + (float)(kBins - 1 - (int)s.bin);
+      need -= s.above;
+      inside = s.inside;
+    }
+    if (inside <= kList) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (i < rounds && place(v[i]) == bin && (!twice || place2(v[i]) == bin2)) {
+          const uint32_t p = (uint32_t)(begin + i * T + tid);
+          // -0 as +0, so that words of equal scores are equal.
+          const uint32_t a = __float_as_uint(v[i] + 0.0f);
+          if constexpr (C == 1) {
+            const uint32_t l = atomicAdd(&s.listed, 1u);
+            s.key[l] = a;
+            s.pos[l] = p;
+          } else {
+            const uint32_t l = peer_add(&s.listed, 0, 1u);
+            peer_store(&s.list_key[l], 0, a);
+            peer_store(&s.list_pos[l], 0, p);
+          }
+        }
+      }
+      row_sync<C>();
+      if constexpr (C > 1) {
+        if (tid < (int)inside) {
+          s.key[tid] = peer_load(&s.list_key[tid], 0);
+          s.pos[tid] = peer_load(&s.list_pos[tid], 0);
+        }
+        __syncthreads();
+      }
+      if (tid < (int)inside) {
+        const float a = __uint_as_float(s.key[tid]);
+        const uint32_t p = s.pos[tid];
+        uint32_t r = 0;
+        for (int j = 0; j < (int)inside; ++j) {
+          const float b = __uint_as_float(s.key[j]);
+          r += b > a || (b == a && s.pos[j] < p) ? 1u : 0u;
+        }
+        if (r + 1 == need) {
+          s.thr_key = s.key[tid];
+          s.thr_pos = p;
+        }
+      }
+      __syncthreads();
+      const float threshold = __uint_as_float(s.thr_key);
+      // Rounds in which an equal score is still taken.
+      const int last = (int)s.thr_pos - begin - tid;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < rounds && (v[i] > threshold || (v[i] == threshold && i * T <= last)))
+          sel |= 1u << i;
+    } else {
+      general = true;
+    }
+  } else {
+    general = true;
+  }
+  if (general) {
+    row_sync<C>();
+    sel = select_general<T, C>(s, x, begin, end, rank, K, &able);
   }
 
   uint32_t at[kPer], base;
