@@ -258,6 +258,7 @@ int sas_kv_append(void* pool, int32_t num_blocks, int32_t block_size, int32_t ro
 /* ---- norm and rotation of rows ---- */
 
 #define SAS_MAX_ROW_DIM 1024
+#define SAS_MAX_ROPE_DIM 256
 
 /* What happens to a row x[0 .. head_dim): its first norm_dim columns are
  * multiplied by rsqrt(mean of their squares + eps) and by norm_weight, then

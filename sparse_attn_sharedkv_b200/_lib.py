@@ -10,6 +10,8 @@ import ctypes as C
 import os
 from typing import Optional
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libsas.so")
 
@@ -24,6 +26,7 @@ PHASE_ATTN, PHASE_COMBINE, PHASE_ALL = 1, 2, 3
 SAS_META_SIZE = 1024
 SAS_NOALLOC_SCRATCH_BYTES = 16 << 20
 SAS_MAX_ROW_DIM = 1024
+SAS_MAX_ROPE_DIM = 256
 SAS_MAX_INDEX_HEADS = 128
 SAS_MAX_INDEX_DIM = 128
 SAS_AIC_CORE_NUM = 36
@@ -180,6 +183,41 @@ def lib() -> C.CDLL:
             fn.argtypes = args
         _LIB = handle
     return _LIB
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+class on_device:
+    """``with on_device(dev) as stream``: dev is the current device, stream its current
+    stream's handle.  Does nothing where dev is current already (a few microseconds that a
+    single-token call would feel)."""
+
+    __slots__ = ("dev", "guard")
+
+    def __init__(self, dev: torch.device):
+        self.dev = dev
+        self.guard = None
+
+    def __enter__(self) -> int:
+        if torch.cuda.current_device() != self.dev.index:
+            self.guard = torch.cuda.device(self.dev)
+            self.guard.__enter__()
+        if _raw_stream is not None:
+            return _raw_stream(self.dev.index)
+        return torch.cuda.current_stream(self.dev).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def dev_i32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """``t`` as a contiguous int32 tensor on ``dev``, itself if it is one."""
+    if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
+        return t
+    return t.to(device=dev, dtype=torch.int32).contiguous()
 
 
 def check(fn: str, code: int) -> None:

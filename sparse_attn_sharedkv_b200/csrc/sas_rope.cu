@@ -11,10 +11,12 @@
 // the other way.  Statistics and products are fp32, rounded once at the end.
 //
 // HBM-bound: every row is read once and written once, as 16-byte vectors.  A
-// group of G lanes (8, 16 or 32 by the row's width) holds a whole row in
+// group of G lanes (8, 16 or 32 by the row's width) holds whole rows in
 // registers, so the mean square is a shuffle reduction inside the group and
-// no shared memory is used; the partner of a column rotated by halves is in
-// another lane and is read a second time (an L1 hit).
+// no shared memory is used.  With many rows a group takes four heads of a
+// token at a time: their loads are in flight together, and the position, the
+// angles and the weights are read once for the four.  The partner of a column
+// rotated by halves is in another lane and is read a second time (an L1 hit).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -74,107 +76,156 @@ __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
   f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
 }
 
-// Columns c .. c + 7 of the row times the norm factor and the weight.
+// Eight weights of a row's columns c .. c + 7.
 template <bool kBf16>
-__device__ __forceinline__ void norm8(const RowArgs& a, int c, float scale, float (&f)[8]) {
-  if (c >= a.norm_dim) return;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] *= scale;
-  if (a.weight != nullptr) {
-    float w[8];
-    if (a.weight_f32)
-      load8(static_cast<const float*>(a.weight) + c, w);
-    else
-      unpack8<kBf16>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.weight) + c)), w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= w[i];
-  }
+__device__ __forceinline__ void load_weight(const RowArgs& a, int c, float (&w)[8]) {
+  if (a.weight_f32)
+    load8(static_cast<const float*>(a.weight) + c, w);
+  else
+    unpack8<kBf16>(
+        __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.weight) + c)), w);
 }
 
-// The row at `src` transformed into `dst` by a group of G lanes (lane `gl`),
-// V vectors of 8 columns each.  `pos`: the rotation position, checked by the
-// caller.  src == dst is allowed: every load of the row is before the
-// group's synchronisation, every store behind it.
-template <int G, int V, bool kBf16>
-__device__ __forceinline__ void transform_row(const RowArgs& a, const uint16_t* src, uint16_t* dst,
-                                              int64_t pos, int gl, uint32_t mask) {
+// `rows` <= R rows at src (src_stride elements apart) transformed into dst by
+// a group of G lanes (lane `gl`), V vectors of 8 columns each.  `pos`: the
+// rows' rotation position, checked by the caller.  src == dst is allowed:
+// every load is before the group's synchronisation, every store behind it.
+// Columns past norm_dim keep a factor of one; at most one of a lane's vectors
+// is rotated (rope_dim <= 8 G).
+template <int G, int V, int R, bool kBf16>
+__device__ __forceinline__ void transform_rows(const RowArgs& a, const uint16_t* src,
+                                               int64_t src_stride, uint16_t* dst,
+                                               int64_t dst_stride, int rows, int64_t pos, int gl,
+                                               uint32_t mask) {
   const int rot0 = a.dim - 2 * a.half;
-  uint4 raw[V], part[V];
-  float4 cs[V][2], sn[V][2];
+  uint4 raw[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (v * G + gl) * 8;
+      raw[r][v] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows && c < a.dim)
+        raw[r][v] = *reinterpret_cast<const uint4*>(src + r * src_stride + c);
+    }
+  // The lane's rotated vector: columns rc .. rc + 7, -1 without one; by
+  // halves its partner is at columns pc.
+  int rc = -1, pc = 0;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int c = (v * G + gl) * 8;
-    raw[v] = make_uint4(0u, 0u, 0u, 0u);
-    if (c < a.dim) {
-      raw[v] = *reinterpret_cast<const uint4*>(src + c);
-      const int rel = c - rot0;
-      if (a.half > 0 && rel >= 0) {
-        if (a.interleaved) {
-          const size_t o = (size_t)pos * a.half + (rel >> 1);
-          cs[v][0] = __ldg(reinterpret_cast<const float4*>(a.cosv + o));
-          sn[v][0] = __ldg(reinterpret_cast<const float4*>(a.sinv + o));
-        } else {
-          const bool low = rel < a.half;
-          part[v] = *reinterpret_cast<const uint4*>(src + (low ? c + a.half : c - a.half));
-          const size_t o = (size_t)pos * a.half + (low ? rel : rel - a.half);
-          cs[v][0] = __ldg(reinterpret_cast<const float4*>(a.cosv + o));
-          cs[v][1] = __ldg(reinterpret_cast<const float4*>(a.cosv + o) + 1);
-          sn[v][0] = __ldg(reinterpret_cast<const float4*>(a.sinv + o));
-          sn[v][1] = __ldg(reinterpret_cast<const float4*>(a.sinv + o) + 1);
+    if (a.half > 0 && c >= rot0 && c < a.dim) rc = c;
+  }
+  float4 cs[2], sn[2];
+  uint4 part[R];
+  const bool low = rc - rot0 < a.half;
+  if (rc >= 0) {
+    const int rel = rc - rot0;
+    if (a.interleaved) {
+      const size_t o = (size_t)pos * a.half + (rel >> 1);
+      cs[0] = __ldg(reinterpret_cast<const float4*>(a.cosv + o));
+      sn[0] = __ldg(reinterpret_cast<const float4*>(a.sinv + o));
+    } else {
+      pc = low ? rc + a.half : rc - a.half;
+      const size_t o = (size_t)pos * a.half + (low ? rel : rel - a.half);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r < rows) part[r] = *reinterpret_cast<const uint4*>(src + r * src_stride + pc);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        cs[i] = __ldg(reinterpret_cast<const float4*>(a.cosv + o) + i);
+        sn[i] = __ldg(reinterpret_cast<const float4*>(a.sinv + o) + i);
+      }
+    }
+  }
+  float scale[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) scale[r] = 1.0f;
+  if (a.norm_dim > 0) {
+    float sum[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if ((v * G + gl) * 8 < a.norm_dim) {
+          float f[8];
+          unpack8<kBf16>(raw[r][v], f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[r] += f[i] * f[i];
         }
       }
     }
-  }
-  float scale = 1.0f;
-  if (a.norm_dim > 0) {
-    float sum = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if ((v * G + gl) * 8 < a.norm_dim) {
-        float f[8];
-        unpack8<kBf16>(raw[v], f);
+    for (int o = G / 2; o > 0; o >>= 1)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += f[i] * f[i];
-      }
-    }
+      for (int r = 0; r < R; ++r) sum[r] += __shfl_xor_sync(mask, sum[r], o);
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
-    scale = rsqrtf(sum * a.inv_n + a.eps);
+    for (int r = 0; r < R; ++r) scale[r] = rsqrtf(sum[r] * a.inv_n + a.eps);
   }
   __syncwarp(mask);
+  // The rows stay packed: unpacked again below rather than kept as floats.
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      asm volatile("" : "+r"(raw[r][v].x), "+r"(raw[r][v].y), "+r"(raw[r][v].z), "+r"(raw[r][v].w));
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int c = (v * G + gl) * 8;
     if (c >= a.dim) continue;
-    float f[8];
-    unpack8<kBf16>(raw[v], f);
-    norm8<kBf16>(a, c, scale, f);
-    const int rel = c - rot0;
-    if (a.half > 0 && rel >= 0) {
-      if (a.interleaved) {
-        const float co[4] = {cs[v][0].x, cs[v][0].y, cs[v][0].z, cs[v][0].w};
-        const float si[4] = {sn[v][0].x, sn[v][0].y, sn[v][0].z, sn[v][0].w};
+    const bool normed = c < a.norm_dim, rotated = c == rc;
+    float w[8], wp[8];
+    const bool weighted = normed && a.weight != nullptr;
+    if (weighted) load_weight<kBf16>(a, c, w);
+    const bool partner = rotated && !a.interleaved;
+    const bool p_weighted = partner && pc < a.norm_dim && a.weight != nullptr;
+    if (p_weighted) load_weight<kBf16>(a, pc, wp);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float s = a.sign * si[i], x0 = f[2 * i], x1 = f[2 * i + 1];
-          f[2 * i] = x0 * co[i] - x1 * s;
-          f[2 * i + 1] = x1 * co[i] + x0 * s;
-        }
-      } else {
-        const bool low = rel < a.half;
-        const float sg = low ? -a.sign : a.sign;
-        float p[8];
-        unpack8<kBf16>(part[v], p);
-        norm8<kBf16>(a, low ? c + a.half : c - a.half, scale, p);
-        const float co[8] = {cs[v][0].x, cs[v][0].y, cs[v][0].z, cs[v][0].w,
-                             cs[v][1].x, cs[v][1].y, cs[v][1].z, cs[v][1].w};
-        const float si[8] = {sn[v][0].x, sn[v][0].y, sn[v][0].z, sn[v][0].w,
-                             sn[v][1].x, sn[v][1].y, sn[v][1].z, sn[v][1].w};
+    for (int r = 0; r < R; ++r) {
+      if (r >= rows) continue;
+      float f[8];
+      unpack8<kBf16>(raw[r][v], f);
+      if (normed) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = f[i] * co[i] + p[i] * (sg * si[i]);
+        for (int i = 0; i < 8; ++i) f[i] *= scale[r];
       }
+      if (weighted) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= w[i];
+      }
+      if (rotated) {
+        if (a.interleaved) {
+          const float co[4] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w};
+          const float si[4] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float s = a.sign * si[i], x0 = f[2 * i], x1 = f[2 * i + 1];
+            f[2 * i] = x0 * co[i] - x1 * s;
+            f[2 * i + 1] = x1 * co[i] + x0 * s;
+          }
+        } else {
+          const float sg = low ? -a.sign : a.sign;
+          float p[8];
+          unpack8<kBf16>(part[r], p);
+          if (pc < a.norm_dim) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] *= scale[r];
+          }
+          if (p_weighted) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] *= wp[i];
+          }
+          const float co[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w,
+                               cs[1].x, cs[1].y, cs[1].z, cs[1].w};
+          const float si[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w,
+                               sn[1].x, sn[1].y, sn[1].z, sn[1].w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * co[i] + p[i] * (sg * si[i]);
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + r * dst_stride + c) = pack8<kBf16>(f);
     }
-    *reinterpret_cast<uint4*>(dst + c) = pack8<kBf16>(f);
   }
 }
 
@@ -193,17 +244,21 @@ struct HeadArgs {
   int32_t* err;
   int64_t x_t, x_h, o_t, o_h;
   int32_t heads;
-  int32_t rows;
+  int32_t chunks;  // of R heads a token
+  int32_t tasks;   // tokens * chunks
   bool pos64;
 };
 
-template <int G, int V, bool kBf16>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(RowArgs a, HeadArgs h) {
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
-  if (row >= h.rows) return;
+// Blocks an SM: registers for the rows in flight, 128 a thread for four rows of
+// up to 768 columns, 64 for one.
+template <int G, int V, int R, bool kBf16>
+__global__ void __launch_bounds__(kThreads, R == 1 ? 4 : V < 4 ? 2 : 1) norm_rope_kernel(RowArgs a, HeadArgs h) {
+  const int64_t task = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
+  if (task >= h.tasks) return;
   const int gl = threadIdx.x & (G - 1);
   const uint32_t mask = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (threadIdx.x & 31 & ~(G - 1));
-  const int t = (int)row / h.heads, head = (int)row - t * h.heads;
+  const int t = (int)task / h.chunks, head = ((int)task - t * h.chunks) * R;
+  const int rows = min(R, h.heads - head);
   int64_t pos = 0;
   uint16_t* dst = h.out + t * h.o_t + head * h.o_h;
   if (a.half > 0) {
@@ -211,12 +266,14 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(RowArgs a, HeadArgs
                   : (long long)__ldg(static_cast<const int32_t*>(h.positions) + t);
     if (pos < 0 || pos >= a.table_rows) {
       if (gl == 0) note_error(h.err, 52, t, head);
-      for (int c = gl * 8; c < a.dim; c += G * 8)
-        *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
+      for (int r = 0; r < rows; ++r)
+        for (int c = gl * 8; c < a.dim; c += G * 8)
+          *reinterpret_cast<uint4*>(dst + r * h.o_h + c) = make_uint4(0u, 0u, 0u, 0u);
       return;
     }
   }
-  transform_row<G, V, kBf16>(a, h.x + t * h.x_t + head * h.x_h, dst, pos, gl, mask);
+  transform_rows<G, V, R, kBf16>(a, h.x + t * h.x_t + head * h.x_h, h.x_h, dst, h.o_h, rows, pos,
+                                 gl, mask);
 }
 
 struct AppendArgs {
@@ -230,7 +287,7 @@ struct AppendArgs {
 };
 
 template <int G, int V, bool kBf16>
-__global__ void __launch_bounds__(kThreads) append_norm_rope_kernel(RowArgs a, AppendArgs p) {
+__global__ void __launch_bounds__(kThreads, 4) append_norm_rope_kernel(RowArgs a, AppendArgs p) {
   const int64_t row64 = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
   if (row64 >= p.total) return;
   const int row = (int)row64;
@@ -264,10 +321,10 @@ __global__ void __launch_bounds__(kThreads) append_norm_rope_kernel(RowArgs a, A
     if (gl == 0) note_error(p.err, 51, row, lo);
     return;
   }
-  transform_row<G, V, kBf16>(
-      a, p.rows + (size_t)row * a.dim,
-      p.pool + ((size_t)blk * p.block_size + (size_t)(pos - lb * p.block_size)) * a.dim, rot, gl,
-      mask);
+  transform_rows<G, V, 1, kBf16>(
+      a, p.rows + (size_t)row * a.dim, 0,
+      p.pool + ((size_t)blk * p.block_size + (size_t)(pos - lb * p.block_size)) * a.dim, 0, 1, rot,
+      gl, mask);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -280,6 +337,7 @@ int row_args(const SasRowTransform* tr, RowArgs* a) {
     return SAS_ERR_INVALID;
   if (tr->rope_dim < 0 || tr->rope_dim > tr->head_dim || tr->rope_dim % 16 != 0)
     return SAS_ERR_INVALID;
+  if (tr->rope_dim > SAS_MAX_ROPE_DIM) return SAS_ERR_UNSUPPORTED;
   if (tr->norm_dim > 0 && !(tr->eps >= 0.0f)) return SAS_ERR_INVALID;
   if (tr->rope_dim > 0 &&
       (!tr->cos || !tr->sin || !aligned16(tr->cos) || !aligned16(tr->sin) || tr->table_rows < 0))
@@ -304,26 +362,45 @@ int row_args(const SasRowTransform* tr, RowArgs* a) {
   return SAS_OK;
 }
 
-// Launches kernel<G, V, bf16> with the group and vectors a lane that hold a
-// row of `dim` columns: the smallest G whose lanes hold it at one vector
-// each, else whole warps at up to 4 vectors a lane.
-#define SAS_ROW_LAUNCH(kernel, G, V, ...)                                                     \
-  do {                                                                                        \
-    const int64_t blocks = (rows + kThreads / (G)-1) / (kThreads / (G));                      \
-    if (bf16)                                                                                 \
-      kernel<G, V, true><<<(unsigned)blocks, kThreads, 0, stream>>>(__VA_ARGS__);             \
-    else                                                                                      \
-      kernel<G, V, false><<<(unsigned)blocks, kThreads, 0, stream>>>(__VA_ARGS__);            \
+// Launches kernel<G, V, ..., bf16> over `tasks` groups, with the group and
+// the vectors a lane that hold a row of `dim` columns: the smallest G whose
+// lanes hold it at one vector each, else whole warps at up to 4 vectors.
+#define SAS_ROW_LAUNCH(G, KERNEL_BF16, KERNEL_FP16, ...)                                  \
+  do {                                                                                    \
+    const unsigned blocks = (unsigned)((tasks + kThreads / (G)-1) / (kThreads / (G)));    \
+    if (bf16)                                                                             \
+      KERNEL_BF16<<<blocks, kThreads, 0, stream>>>(__VA_ARGS__);                          \
+    else                                                                                  \
+      KERNEL_FP16<<<blocks, kThreads, 0, stream>>>(__VA_ARGS__);                          \
   } while (0)
-#define SAS_ROW_DISPATCH(kernel, ...)                                                         \
-  do {                                                                                        \
-    if (dim <= 64) SAS_ROW_LAUNCH(kernel, 8, 1, __VA_ARGS__);                                 \
-    else if (dim <= 128) SAS_ROW_LAUNCH(kernel, 16, 1, __VA_ARGS__);                          \
-    else if (dim <= 256) SAS_ROW_LAUNCH(kernel, 32, 1, __VA_ARGS__);                          \
-    else if (dim <= 512) SAS_ROW_LAUNCH(kernel, 32, 2, __VA_ARGS__);                          \
-    else if (dim <= 768) SAS_ROW_LAUNCH(kernel, 32, 3, __VA_ARGS__);                          \
-    else SAS_ROW_LAUNCH(kernel, 32, 4, __VA_ARGS__);                                          \
-  } while (0)
+
+template <int R>
+void launch_heads(const RowArgs& a, const HeadArgs& h, bool bf16, cudaStream_t stream) {
+  const int64_t tasks = h.tasks;
+#define SAS_HEADS(G, V) \
+  SAS_ROW_LAUNCH(G, (norm_rope_kernel<G, V, R, true>), (norm_rope_kernel<G, V, R, false>), a, h)
+  if (a.dim <= 64) SAS_HEADS(8, 1);
+  else if (a.dim <= 128) SAS_HEADS(16, 1);
+  else if (a.dim <= 256) SAS_HEADS(32, 1);
+  else if (a.dim <= 512) SAS_HEADS(32, 2);
+  else if (a.dim <= 768) SAS_HEADS(32, 3);
+  else SAS_HEADS(32, 4);
+#undef SAS_HEADS
+}
+
+void launch_append(const RowArgs& a, const AppendArgs& p, bool bf16, cudaStream_t stream) {
+  const int64_t tasks = p.total;
+#define SAS_APPEND(G, V)                                                                    \
+  SAS_ROW_LAUNCH(G, (append_norm_rope_kernel<G, V, true>), (append_norm_rope_kernel<G, V, false>), \
+                 a, p)
+  if (a.dim <= 64) SAS_APPEND(8, 1);
+  else if (a.dim <= 128) SAS_APPEND(16, 1);
+  else if (a.dim <= 256) SAS_APPEND(32, 1);
+  else if (a.dim <= 512) SAS_APPEND(32, 2);
+  else if (a.dim <= 768) SAS_APPEND(32, 3);
+  else SAS_APPEND(32, 4);
+#undef SAS_APPEND
+}
 
 }  // namespace
 
@@ -343,13 +420,23 @@ extern "C" int sas_norm_rope(const SasRowTransform* tr, const void* x, int64_t x
   if (!aligned16(x) || !aligned16(out) || (x_stride_token | x_stride_head | out_stride_token |
                                            out_stride_head) % 8 != 0)
     return SAS_ERR_INVALID;
+  // Four heads a group where that still leaves every SM sixteen warps or more;
+  // fewer rows are spread one a group for the shortest time.
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return SAS_ERR_CUDA;
+  const int per = heads >= 4 && rows / 4 >= 16 * (int64_t)sms ? 4 : 1;
+  const int chunks = (heads + per - 1) / per;
   const HeadArgs h{static_cast<const uint16_t*>(x), static_cast<uint16_t*>(out), positions, err,
-                   x_stride_token, x_stride_head, out_stride_token, out_stride_head, heads,
-                   (int32_t)rows, positions_i64 != 0};
+                   x_stride_token, x_stride_head, out_stride_token, out_stride_head, heads, chunks,
+                   tokens * chunks, positions_i64 != 0};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const bool bf16 = tr->dtype == SAS_DTYPE_BF16;
-  const int dim = a.dim;
-  SAS_ROW_DISPATCH(norm_rope_kernel, a, h);
+  if (per == 4)
+    launch_heads<4>(a, h, bf16, stream);
+  else
+    launch_heads<1>(a, h, bf16, stream);
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
 
@@ -372,9 +459,6 @@ extern "C" int sas_kv_append_norm_rope(const SasRowTransform* tr, void* pool, in
                      block_table, cu_new, start_pos, err, num_blocks, block_size, table_len, batch,
                      total_new, cmp_ratio};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  const bool bf16 = tr->dtype == SAS_DTYPE_BF16;
-  const int64_t rows = total_new;
-  const int dim = a.dim;
-  SAS_ROW_DISPATCH(append_norm_rope_kernel, a, p);
+  launch_append(a, p, tr->dtype == SAS_DTYPE_BF16, stream);
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }

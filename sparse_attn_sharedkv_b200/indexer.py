@@ -22,13 +22,12 @@ captured in a CUDA graph.  No CPU fallback, no backward pass.
 
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from .api import _check_device_errors, _dev_i32, _dtype_code
+from .api import _check_device_errors, _dtype_code
 
 # Bytes of scores that select_keys holds at a time: well inside the 126 MB L2,
 # so that the selection reads them back from there.
@@ -40,25 +39,25 @@ def _index_params(q, weights, key_pool, block_table, cu_seqlens_q, seqused_kv, c
     """Validate the arguments; returns the C struct (without outputs), the
     number of columns and the tensors the struct points to."""
     code = _dtype_code(q.dtype)
-    dev = q.device
+    dev, shape = q.device, q.shape
     if dev.type != "cuda":
         raise RuntimeError(f"index scores run on a CUDA (sm_100a) device only; got q on {dev}")
     if layout_q == "TND":
-        if q.dim() != 3:
-            raise ValueError(f"q must be [T, H, D] in TND (got {tuple(q.shape)})")
+        if len(shape) != 3:
+            raise ValueError(f"q must be [T, H, D] in TND (got {tuple(shape)})")
         if cu_seqlens_q is None:
             raise ValueError("cu_seqlens_q is required for TND")
-        total, S, B = q.shape[0], 0, cu_seqlens_q.numel() - 1
+        total, S, B = shape[0], 0, cu_seqlens_q.numel() - 1
     elif layout_q == "BSND":
-        if q.dim() != 4:
-            raise ValueError(f"q must be [B, S, H, D] in BSND (got {tuple(q.shape)})")
-        B, S = q.shape[:2]
+        if len(shape) != 4:
+            raise ValueError(f"q must be [B, S, H, D] in BSND (got {tuple(shape)})")
+        B, S = shape[0], shape[1]
         total = B * S
         if cu_seqlens_q is not None and cu_seqlens_q.numel() != B + 1:
             raise ValueError("cu_seqlens_q must have B + 1 entries")
     else:
         raise ValueError(f"unsupported layout_q={layout_q!r}")
-    H, D = q.shape[-2:]
+    H, D = shape[-2], shape[-1]
     if not 1 <= H <= _lib.SAS_MAX_INDEX_HEADS:
         raise ValueError(f"index heads must be in [1, {_lib.SAS_MAX_INDEX_HEADS}] (got {H})")
     if D % 8 or not 8 <= D <= _lib.SAS_MAX_INDEX_DIM:
@@ -66,37 +65,38 @@ def _index_params(q, weights, key_pool, block_table, cu_seqlens_q, seqused_kv, c
                          f"{_lib.SAS_MAX_INDEX_DIM} (got {D})")
     if B < 1 and total > 0:
         raise ValueError("at least one sequence is needed")
-    if weights.shape != q.shape[:-1] or weights.dtype != torch.float32:
+    if weights.shape != shape[:-1] or weights.dtype is not torch.float32:
         raise ValueError("weights must be float32 of q's shape without the last dim")
-    if key_pool.dim() not in (3, 4) or (key_pool.dim() == 4 and key_pool.shape[2] != 1):
+    pool_shape = key_pool.shape
+    if len(pool_shape) not in (3, 4) or (len(pool_shape) == 4 and pool_shape[2] != 1):
         raise ValueError("key_pool must be [blocks, block_size, 1, D]")
-    if key_pool.shape[-1] != D or key_pool.dtype != q.dtype:
+    if pool_shape[-1] != D or key_pool.dtype is not q.dtype:
         raise ValueError("q and key_pool must share the head dim and the dtype")
-    if key_pool.shape[1] < 1:
+    if pool_shape[1] < 1:
         raise ValueError("block_size must be >= 1")
-    if key_pool.shape[0] * key_pool.shape[1] > 2 ** 31 - 1:
-        raise ValueError("key_pool holds more than 2^31 - 1 rows")
-    if block_table.dim() != 2 or block_table.shape[0] < B:
+    if pool_shape[0] * pool_shape[1] > 2 ** 31 - 2:
+        raise ValueError("key_pool holds more than 2^31 - 2 rows")
+    table_shape = block_table.shape
+    if len(table_shape) != 2 or table_shape[0] < B:
         raise ValueError("block_table must be [B, table_len]")
     if seqused_kv.numel() < B:
         raise ValueError("seqused_kv must have one entry per sequence")
-    for name, t in (("weights", weights), ("key_pool", key_pool)):
-        if t.device != dev:
-            raise ValueError(f"{name} must be on q's device")
+    if weights.device != dev or key_pool.device != dev:
+        raise ValueError("weights and key_pool must be on q's device")
     if cmp_ratio < 1:
         raise ValueError(f"cmp_ratio must be >= 1 (got {cmp_ratio})")
-    N = block_table.shape[1] * key_pool.shape[1] if max_keys is None else int(max_keys)
+    N = table_shape[1] * pool_shape[1] if max_keys is None else int(max_keys)
     if not 0 <= N <= 2 ** 31 - 1024:
         raise ValueError(f"max_keys out of range ({N})")
     qf, w, pool = q.contiguous(), weights.contiguous(), key_pool.contiguous()
-    bt, kv = _dev_i32(block_table, dev), _dev_i32(seqused_kv, dev)
-    cu = _dev_i32(cu_seqlens_q, dev) if cu_seqlens_q is not None else None
+    if (qf.data_ptr() | pool.data_ptr()) & 15:
+        raise ValueError("q and key_pool must be 16-byte aligned")
+    bt, kv = _lib.dev_i32(block_table, dev), _lib.dev_i32(seqused_kv, dev)
+    cu = _lib.dev_i32(cu_seqlens_q, dev) if cu_seqlens_q is not None else None
     p = _lib.SasIndexParams(
-        q=qf.data_ptr(), weights=w.data_ptr(), key_pool=pool.data_ptr(),
-        block_table=bt.data_ptr(), cu_seqlens_q=cu.data_ptr() if cu is not None else None,
-        kv_len=kv.data_ptr(), batch=B, total_tokens=total, max_q_len=S, num_heads=H, head_dim=D,
-        dtype=code, block_size=pool.shape[1], num_blocks=pool.shape[0], table_len=bt.shape[1],
-        cmp_ratio=int(cmp_ratio), num_keys=N)
+        qf.data_ptr(), w.data_ptr(), pool.data_ptr(), bt.data_ptr(),
+        cu.data_ptr() if cu is not None else None, kv.data_ptr(), None, None, None, B, total, S, H,
+        D, code, pool_shape[1], pool_shape[0], table_shape[1], int(cmp_ratio), N)
     return p, N, (qf, w, pool, bt, kv, cu)
 
 
@@ -141,9 +141,8 @@ def index_scores(q: torch.Tensor, weights: torch.Tensor, *, key_pool: torch.Tens
         p.lengths = lengths.data_ptr() if lengths is not None else None
         p.err = err.data_ptr() if err is not None else None
         p.first_token, p.num_tokens, p.fill = 0, total, 1
-        with torch.cuda.device(dev):
-            _lib.check("sas_index_scores", _lib.lib().sas_index_scores(
-                C.byref(p), torch.cuda.current_stream(dev).cuda_stream))
+        with _lib.on_device(dev) as stream:
+            _lib.check("sas_index_scores", _lib.lib().sas_index_scores(p, stream))
         if err is not None:
             _raise_device_error(err)
     del keep
@@ -166,26 +165,31 @@ def select_topk(scores: torch.Tensor, topk: int, *,
     dev = scores.device
     if dev.type != "cuda":
         raise RuntimeError(f"select_topk runs on a CUDA (sm_100a) device only; got {dev}")
-    if scores.dtype != torch.float32 or scores.dim() not in (2, 3):
+    shape, topk = scores.shape, int(topk)
+    if scores.dtype is not torch.float32 or len(shape) not in (2, 3):
         raise ValueError("scores must be float32 [T, N] or [B, S, N]")
     if topk < 1:
         raise ValueError(f"topk must be >= 1 (got {topk})")
-    lead, N = scores.shape[:-1], scores.shape[-1]
-    rows = lead.numel()
-    out = torch.empty((*lead, 1, topk), dtype=torch.int32, device=dev)
+    N = shape[-1]
+    rows = shape[0] if len(shape) == 2 else shape[0] * shape[1]
+    if rows > (2 ** 31 - 1) // 8:
+        raise ValueError("scores hold more than 2^28 - 1 rows")
+    out = torch.empty((*shape[:-1], 1, topk), dtype=torch.int32, device=dev)
     if lengths is not None:
         if lengths.numel() != rows:
             raise ValueError("lengths must have one entry per row of scores")
-        lengths = _dev_i32(lengths, dev)
+        lengths = _lib.dev_i32(lengths, dev)
     if rows == 0:
         return out
-    x = scores.reshape(rows, N)
-    if N > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < N:
+    x = scores if len(shape) == 2 else scores.reshape(rows, N)
+    row_stride, col_stride = x.stride()
+    if (N > 1 and col_stride != 1) or (rows > 1 and row_stride < N):
         x = x.contiguous()
-    with torch.cuda.device(dev):
+        row_stride = N
+    with _lib.on_device(dev) as stream:
         _lib.check("sas_topk_select", _lib.lib().sas_topk_select(
-            x.data_ptr(), max(x.stride(0), N), lengths.data_ptr() if lengths is not None else None,
-            rows, N, int(topk), out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
+            x.data_ptr(), max(row_stride, N), lengths.data_ptr() if lengths is not None else None,
+            rows, N, topk, out.data_ptr(), stream))
     return out
 
 
@@ -201,6 +205,7 @@ def select_keys(q: torch.Tensor, weights: torch.Tensor, *, key_pool: torch.Tenso
     """
     p, N, keep = _index_params(q, weights, key_pool, block_table, cu_seqlens_q, seqused_kv,
                                cmp_ratio, layout_q, max_keys)
+    topk = int(topk)
     if topk < 1:
         raise ValueError(f"topk must be >= 1 (got {topk})")
     dev, total = q.device, p.total_tokens
@@ -215,13 +220,12 @@ def select_keys(q: torch.Tensor, weights: torch.Tensor, *, key_pool: torch.Tenso
     p.scores, p.score_stride, p.lengths, p.fill = scores.data_ptr(), stride, lengths.data_ptr(), 0
     p.err = err.data_ptr() if err is not None else None
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
+    with _lib.on_device(dev) as stream:
         for t in range(0, total, part):
             p.first_token, p.num_tokens = t, min(part, total - t)
-            _lib.check("sas_index_scores", L.sas_index_scores(C.byref(p), stream))
+            _lib.check("sas_index_scores", L.sas_index_scores(p, stream))
             _lib.check("sas_topk_select", L.sas_topk_select(
-                scores.data_ptr(), stride, lengths.data_ptr(), p.num_tokens, N, int(topk),
+                scores.data_ptr(), stride, lengths.data_ptr(), p.num_tokens, N, topk,
                 out.data_ptr() + 4 * t * topk, stream))
     if err is not None:
         _raise_device_error(err)

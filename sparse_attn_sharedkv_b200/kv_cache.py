@@ -96,20 +96,22 @@ def append_paged_kv_norm_rope(kv_pool: torch.Tensor, block_table: torch.Tensor,
     dev = kv_pool.device
     if dev.type != "cuda" or new_rows.device != dev:
         raise RuntimeError("kv_pool and new_rows must be on one CUDA (sm_100a) device")
-    if kv_pool.dim() not in (3, 4) or (kv_pool.dim() == 4 and kv_pool.shape[2] != 1):
+    pool_shape = kv_pool.shape
+    if len(pool_shape) not in (3, 4) or (len(pool_shape) == 4 and pool_shape[2] != 1):
         raise ValueError("kv_pool must be [blocks, block_size, 1, D]")
-    D = kv_pool.shape[-1]
+    D = pool_shape[-1]
     if new_rows.dtype != kv_pool.dtype or new_rows.shape[-1] != D:
         raise ValueError("new_rows must have the pool's dtype and last dim")
     if not kv_pool.is_contiguous() or not new_rows.is_contiguous():
         raise ValueError("kv_pool and new_rows must be contiguous")
-    if kv_pool.shape[1] < 1:
+    if pool_shape[1] < 1:
         raise ValueError("block_size must be >= 1")
-    if block_table.dim() != 2 or block_table.shape[0] < 1:
+    table_shape = block_table.shape
+    if len(table_shape) != 2 or table_shape[0] < 1:
         raise ValueError("block_table must be [B, table_len] with B >= 1")
     if cmp_ratio < 1:
         raise ValueError(f"cmp_ratio must be >= 1 (got {cmp_ratio})")
-    B = block_table.shape[0]
+    B = table_shape[0]
     if cu_seqlens_new.numel() != B + 1 or start_pos.numel() != B:
         raise ValueError("cu_seqlens_new must have B + 1 entries and start_pos B")
     tr = row_transform(kv_pool.dtype, dev, D, cos, sin, int(norm_dim), norm_weight, eps,
@@ -117,16 +119,17 @@ def append_paged_kv_norm_rope(kv_pool: torch.Tensor, block_table: torch.Tensor,
     total = new_rows.numel() // D
     if total == 0:
         return None
-    bt = block_table.to(device=dev, dtype=torch.int32).contiguous()
-    cu = cu_seqlens_new.to(device=dev, dtype=torch.int32).contiguous()
-    sp = start_pos.to(device=dev, dtype=torch.int32).contiguous()
+    if (kv_pool.data_ptr() | new_rows.data_ptr()) & 15:
+        raise ValueError("kv_pool and new_rows must be 16-byte aligned")
+    bt = _lib.dev_i32(block_table, dev)
+    cu = _lib.dev_i32(cu_seqlens_new, dev)
+    sp = _lib.dev_i32(start_pos, dev)
     err = torch.zeros(4, dtype=torch.int32, device=dev) if check_errors else None
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev) as stream:
         _lib.check("sas_kv_append_norm_rope", _lib.lib().sas_kv_append_norm_rope(
-            C.byref(tr), kv_pool.data_ptr(), kv_pool.shape[0], kv_pool.shape[1], bt.data_ptr(),
-            bt.shape[1], new_rows.data_ptr(), cu.data_ptr(), sp.data_ptr(), B, total,
-            int(cmp_ratio), err.data_ptr() if err is not None else None,
-            torch.cuda.current_stream(dev).cuda_stream))
+            tr, kv_pool.data_ptr(), pool_shape[0], pool_shape[1], bt.data_ptr(), table_shape[1],
+            new_rows.data_ptr(), cu.data_ptr(), sp.data_ptr(), B, total, int(cmp_ratio),
+            err.data_ptr() if err is not None else None, stream))
     if err is not None:
         e = err.tolist()
         return e if e[0] != 0 else None

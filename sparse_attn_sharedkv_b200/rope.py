@@ -15,7 +15,6 @@ CPU fallback and no backward pass.
 
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional
 
 import torch
@@ -37,53 +36,64 @@ def row_transform(dtype, device, head_dim, cos, sin, norm_dim, norm_weight, eps,
                          f"(got {head_dim})")
     if norm_dim % 8 or not 0 <= norm_dim <= head_dim:
         raise ValueError(f"norm_dim must be a multiple of 8 in [0, {head_dim}] (got {norm_dim})")
-    tr = _lib.SasRowTransform(head_dim=head_dim, norm_dim=norm_dim, dtype=code,
-                              interleaved=bool(interleaved), inverse=bool(inverse), eps=eps)
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
+    cos_ptr = sin_ptr = weight_ptr = None
+    rows = rope_dim = weight_code = 0
     if cos is not None:
-        if cos.dim() != 2 or cos.shape != sin.shape:
+        shape = cos.shape
+        if len(shape) != 2 or shape != sin.shape:
             raise ValueError("cos and sin must be [positions, rope_dim / 2]")
-        rope_dim = 2 * cos.shape[1]
-        if rope_dim % 16 or not 16 <= rope_dim <= head_dim:
-            raise ValueError(f"rope_dim must be a multiple of 16 up to {head_dim} "
-                             f"(got {rope_dim})")
+        rows, rope_dim = min(shape[0], 2 ** 31 - 1), 2 * shape[1]
+        if rope_dim % 16 or not 16 <= rope_dim <= min(head_dim, _lib.SAS_MAX_ROPE_DIM):
+            raise ValueError(f"rope_dim must be a multiple of 16 up to "
+                             f"{min(head_dim, _lib.SAS_MAX_ROPE_DIM)} (got {rope_dim})")
         for name, t in (("cos", cos), ("sin", sin)):
-            if t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+            if t.dtype is not torch.float32 or t.device != device or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous float32 tensor on {device}")
-        tr.cos, tr.sin = cos.data_ptr(), sin.data_ptr()
-        tr.table_rows, tr.rope_dim = min(cos.shape[0], 2 ** 31 - 1), rope_dim
+        cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
+        if (cos_ptr | sin_ptr) & 15:
+            raise ValueError("cos and sin must be 16-byte aligned")
     if norm_weight is not None:
         if norm_weight.shape != (norm_dim,):
             raise ValueError(f"norm_weight must be [norm_dim] = [{norm_dim}]")
-        if norm_weight.dtype not in (torch.float32, dtype) or norm_weight.device != device \
+        wt = norm_weight.dtype
+        if (wt is not torch.float32 and wt is not dtype) or norm_weight.device != device \
                 or not norm_weight.is_contiguous():
             raise ValueError(f"norm_weight must be contiguous, float32 or {dtype}, on {device}")
-        tr.norm_weight = norm_weight.data_ptr() if norm_dim else None
-        tr.weight_dtype = _lib.DTYPE_F32 if norm_weight.dtype == torch.float32 else code
+        if norm_dim:
+            weight_ptr = norm_weight.data_ptr()
+            if weight_ptr & 15:
+                raise ValueError("norm_weight must be 16-byte aligned")
+        weight_code = _lib.DTYPE_F32 if wt is torch.float32 else code
     if norm_dim == 0 and cos is None:
         raise ValueError("nothing to do: neither a norm nor a rotation is asked for")
-    return tr
+    if norm_dim and not eps >= 0:
+        raise ValueError(f"eps must not be negative (got {eps})")
+    return _lib.SasRowTransform(cos_ptr, sin_ptr, weight_ptr, rows, head_dim, norm_dim, rope_dim,
+                                code, weight_code, bool(interleaved), bool(inverse), eps)
 
 
-def _head_rows(t: torch.Tensor) -> Optional[torch.Tensor]:
-    """[T, H, D] view of [..., H, D] that the kernel can address, or None."""
-    try:
-        v = t.view(-1, t.shape[-2], t.shape[-1])
-    except RuntimeError:
-        return None
-    ok = (v.stride(2) == 1 and v.stride(0) % 8 == 0 and v.stride(1) % 8 == 0
-          and v.data_ptr() % 16 == 0)
-    return v if ok else None
+def _head_rows(t: torch.Tensor):
+    """(data pointer, token stride, head stride) by which the kernel can
+    address [..., H, D] ``t`` as [T, H, D], or None."""
+    if t.dim() == 4:
+        try:
+            t = t.view(-1, t.shape[-2], t.shape[-1])
+        except RuntimeError:
+            return None
+    st, sh, sd = t.stride()
+    ptr = t.data_ptr()
+    return (ptr, st, sh) if sd == 1 and not (st | sh) & 7 and not ptr & 15 else None
 
 
-def _rows_overlap(v: torch.Tensor) -> bool:
-    """Whether rows of the [T, H, D] view share memory."""
-    end = v.shape[2]
-    for stride, size in sorted(zip(v.stride()[:2], v.shape[:2])):
+def _rows_overlap(sizes, strides, width: int) -> bool:
+    """Whether rows of ``width`` elements at these sizes and strides share memory."""
+    end = width
+    for stride, size in sorted(zip(strides, sizes)):
         if size > 1 and stride < end:
             return True
-        end = stride * (size - 1) + end
+        end += stride * (size - 1)
     return False
 
 
@@ -113,39 +123,44 @@ def norm_rope(x: torch.Tensor, positions: Optional[torch.Tensor] = None,
     dev = x.device
     if dev.type != "cuda":
         raise RuntimeError(f"norm_rope runs on a CUDA (sm_100a) device only; got x on {dev}")
-    if x.dim() not in (3, 4):
-        raise ValueError(f"x must be [T, H, D] or [B, S, H, D] (got {tuple(x.shape)})")
-    H, D = x.shape[-2], x.shape[-1]
+    shape = x.shape
+    if len(shape) not in (3, 4):
+        raise ValueError(f"x must be [T, H, D] or [B, S, H, D] (got {tuple(shape)})")
+    H, D = shape[-2], shape[-1]
     tr = row_transform(x.dtype, dev, D, cos, sin, int(norm_dim), norm_weight, eps, interleaved,
                        inverse)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != dev:
-        raise ValueError("out must have x's shape, dtype and device")
-    T = x.numel() // (H * D) if x.numel() else 0
-    pos = None
-    if tr.rope_dim:
+    T = shape[0] if len(shape) == 3 else shape[0] * shape[1]
+    if T * H > 2 ** 31 - 1:
+        raise ValueError("x holds more than 2^31 - 1 rows")
+    pos_ptr, pos64 = None, 0
+    if cos is not None:
         if positions is None or positions.dtype not in (torch.int32, torch.int64) \
-                or positions.numel() != x.shape[:-2].numel():
+                or positions.numel() != T:
             raise ValueError("positions must be int32 or int64 with one entry per token")
-        pos = positions.to(dev).contiguous()
-    if T == 0:
+        if positions.device != dev or not positions.is_contiguous():
+            positions = positions.to(dev).contiguous()
+        pos_ptr, pos64 = positions.data_ptr(), positions.dtype is torch.int64
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        o = (out.data_ptr(), H * D, D)
+    else:
+        if out.shape != shape or out.dtype != x.dtype or out.device != dev:
+            raise ValueError("out must have x's shape, dtype and device")
+        o = _head_rows(out)
+        if T * H > 0 and (o is None or _rows_overlap((T, H), o[1:], D)):
+            raise ValueError("out must have a contiguous last dim, strides of multiples of 8, "
+                             "16-byte alignment and rows that do not overlap")
+    if T * H == 0:
         return out
-    o = _head_rows(out)
-    if o is None or _rows_overlap(o):
-        raise ValueError("out must have a contiguous last dim, strides of multiples of 8, "
-                         "16-byte alignment and rows that do not overlap")
     v = _head_rows(x)
     if v is None:
-        v = x.reshape(T, H, D).clone(memory_format=torch.contiguous_format)
+        x = x.clone(memory_format=torch.contiguous_format)
+        v = (x.data_ptr(), H * D, D)
     err = torch.zeros(4, dtype=torch.int32, device=dev) if check_errors else None
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev) as stream:
         _lib.check("sas_norm_rope", _lib.lib().sas_norm_rope(
-            C.byref(tr), v.data_ptr(), v.stride(0), v.stride(1), o.data_ptr(), o.stride(0),
-            o.stride(1), T, H, pos.data_ptr() if pos is not None else None,
-            int(pos is not None and pos.dtype == torch.int64),
-            err.data_ptr() if err is not None else None,
-            torch.cuda.current_stream(dev).cuda_stream))
+            tr, *v, *o, T, H, pos_ptr, pos64, err.data_ptr() if err is not None else None,
+            stream))
     if err is not None:
         e = err.tolist()
         if e[0]:

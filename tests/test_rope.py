@@ -72,6 +72,9 @@ def check(got, want, mag, dtype):
     (dict(norm_weight=torch.ones(8)), "norm_weight"),
     (dict(norm_weight=torch.ones(512, dtype=torch.float16)), "norm_weight"),
     (dict(norm_dim=0, norm_weight=None, cos=None, sin=None), "nothing to do"),
+    (dict(head_dim=1024, cos=torch.zeros(8, 144), sin=torch.zeros(8, 144)), "rope_dim"),
+    (dict(cos=tables(64, 8)[0].view(-1)[2:34].view(1, 32), sin=torch.zeros(1, 32)), "aligned"),
+    (dict(eps=-1.0), "eps"),
 ])
 def test_transform_refuses(change, word):
     cos, sin = tables(64, 8)
@@ -123,11 +126,9 @@ def test_entry_points_refuse_without_a_launch():
 
 
 def test_rows_overlap():
-    t = torch.zeros(4, 3, 16)
-    assert not _rows_overlap(t) and not _rows_overlap(t.transpose(0, 1))
-    assert not _rows_overlap(t[:, :1]) and not _rows_overlap(t[..., :8])
-    assert _rows_overlap(t[:1].expand(4, 3, 16))
-    assert _rows_overlap(torch.zeros(100).as_strided((2, 3, 16), (16, 16, 1)))
+    assert not _rows_overlap((4, 3), (48, 16), 16) and not _rows_overlap((3, 4), (16, 48), 16)
+    assert not _rows_overlap((4, 1), (48, 0), 16) and not _rows_overlap((4, 3), (48, 16), 8)
+    assert _rows_overlap((4, 3), (0, 16), 16) and _rows_overlap((2, 3), (16, 16), 16)
 
 
 # ---- on a GPU ----
