@@ -10,13 +10,13 @@
 // halves, with (cos, sin) from tables [positions, rope / 2]; `inverse` turns
 // the other way.  Statistics and products are fp32, rounded once at the end.
 //
-// HBM-bound: every row is read once and written once, as 16-byte vectors.  A
-// group of G lanes (8, 16 or 32 by the row's width) holds whole rows in
-// registers, so the mean square is a shuffle reduction inside the group and
-// no shared memory is used.  With many rows a group takes four heads of a
-// token at a time: their loads are in flight together, and the position, the
-// angles and the weights are read once for the four.  The partner of a column
-// rotated by halves is in another lane and is read a second time (an L1 hit).
+// HBM-bound: every row is read once and written once, as 16-byte vectors.
+// Eight lanes hold a whole row in registers, V vectors each (9 of them for 576
+// columns, with no lane idle), four rows a warp: all of a row's loads are in
+// flight together, the mean square takes three shuffles, and what a row costs
+// besides (its token, position and address) is shared by four.  The rotated
+// columns are taken apart from the others, a lane with both columns of its
+// pairs, so no lane needs another's.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,6 +28,7 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kLanes = 8;  // of a row
 
 struct RowArgs {
   const float* cosv;
@@ -38,195 +39,206 @@ struct RowArgs {
   bool weight_f32, interleaved;
 };
 
-template <bool kBf16>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 p;
-    if constexpr (kBf16)
-      p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-    else
-      p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    f[2 * i] = p.x;
-    f[2 * i + 1] = p.y;
-  }
+// Pairs of fp32 in one 64-bit register: one instruction multiplies or adds both.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
+// Eight columns as four pairs.
+struct Eight {
+  uint64_t p[4];
+};
+
 template <bool kBf16>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint32_t w[4];
+__device__ __forceinline__ Eight unpack8(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  Eight e;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (kBf16) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      e.p[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      e.p[i] = pair(f.x, f.y);
+    }
+  }
+  return e;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint4 pack8(const Eight& e) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpair(e.p[i]);
+    if constexpr (kBf16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     } else {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      const __half2 h = __floats2half2_rn(f.x, f.y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-  const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-  f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-}
-
-// Eight weights of a row's columns c .. c + 7.
+// Weights of a row's columns c .. c + 7 < norm_dim.
 template <bool kBf16>
-__device__ __forceinline__ void load_weight(const RowArgs& a, int c, float (&w)[8]) {
-  if (a.weight_f32)
-    load8(static_cast<const float*>(a.weight) + c, w);
-  else
-    unpack8<kBf16>(
-        __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.weight) + c)), w);
+__device__ __forceinline__ Eight load_weight(const RowArgs& a, int c) {
+  if (!a.weight_f32)
+    return unpack8<kBf16>(
+        __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.weight) + c)));
+  const float4* w = reinterpret_cast<const float4*>(static_cast<const float*>(a.weight) + c);
+  const float4 x = __ldg(w), y = __ldg(w + 1);
+  return Eight{{pair(x.x, x.y), pair(x.z, x.w), pair(y.x, y.y), pair(y.z, y.w)}};
 }
 
-// `rows` <= R rows at src (src_stride elements apart) transformed into dst by
-// a group of G lanes (lane `gl`), V vectors of 8 columns each.  `pos`: the
-// rows' rotation position, checked by the caller.  src == dst is allowed:
-// every load is before the group's synchronisation, every store behind it.
-// Columns past norm_dim keep a factor of one; at most one of a lane's vectors
-// is rotated (rope_dim <= 8 G).
-template <int G, int V, int R, bool kBf16>
-__device__ __forceinline__ void transform_rows(const RowArgs& a, const uint16_t* src,
-                                               int64_t src_stride, uint16_t* dst,
-                                               int64_t dst_stride, int rows, int64_t pos, int gl,
-                                               uint32_t mask) {
-  const int rot0 = a.dim - 2 * a.half;
-  uint4 raw[R][V];
+// Columns c .. c + 7 normed and weighted.
+template <bool kBf16, bool kWeighted>
+__device__ __forceinline__ Eight norm8(const RowArgs& a, const uint4& raw, float scale, int c) {
+  Eight e = unpack8<kBf16>(raw);
+  if (c < a.norm_dim) {
+    const uint64_t k = pair(scale, scale);
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+    for (int i = 0; i < 4; ++i) e.p[i] = mul2(e.p[i], k);
+    if constexpr (kWeighted) {
+      const Eight w = load_weight<kBf16>(a, c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e.p[i] = mul2(e.p[i], w.p[i]);
+    }
+  }
+  return e;
+}
+
+// Rotated columns of one lane: eight neighbouring ones (interleaved), or eight
+// of the first half and their partners of the second.
+struct Turn {
+  int c;  // first column, -1 for none
+  uint4 x, y;
+  float4 cs[2], sn[2];
+};
+
+__device__ __forceinline__ Turn load_turn(const RowArgs& a, const uint16_t* src, int64_t pos,
+                                          int i) {
+  const int rot0 = a.dim - 2 * a.half;
+  Turn t;
+  t.c = 8 * i < (a.interleaved ? 2 * a.half : a.half) ? rot0 + 8 * i : -1;
+  if (t.c >= 0) {
+    const size_t o = (size_t)pos * a.half + (a.interleaved ? 4 * i : 8 * i);
+    const float4* cp = reinterpret_cast<const float4*>(a.cosv + o);
+    const float4* sp = reinterpret_cast<const float4*>(a.sinv + o);
+    t.x = *reinterpret_cast<const uint4*>(src + t.c);
+    t.cs[0] = __ldg(cp);
+    t.sn[0] = __ldg(sp);
+    if (!a.interleaved) {
+      t.y = *reinterpret_cast<const uint4*>(src + t.c + a.half);
+      t.cs[1] = __ldg(cp + 1);
+      t.sn[1] = __ldg(sp + 1);
+    }
+  }
+  return t;
+}
+
+template <bool kBf16, bool kWeighted>
+__device__ __forceinline__ void store_turn(const RowArgs& a, const Turn& t, uint16_t* dst,
+                                           float scale) {
+  if (t.c < 0) return;
+  Eight e = norm8<kBf16, kWeighted>(a, t.x, scale, t.c);
+  if (a.interleaved) {
+    const float co[4] = {t.cs[0].x, t.cs[0].y, t.cs[0].z, t.cs[0].w};
+    const float si[4] = {t.sn[0].x, t.sn[0].y, t.sn[0].z, t.sn[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpair(e.p[i]);
+      const float s = a.sign * si[i];
+      e.p[i] = pair(f.x * co[i] - f.y * s, f.y * co[i] + f.x * s);
+    }
+  } else {
+    Eight q = norm8<kBf16, kWeighted>(a, t.y, scale, t.c + a.half);
+    const uint64_t co[4] = {pair(t.cs[0].x, t.cs[0].y), pair(t.cs[0].z, t.cs[0].w),
+                            pair(t.cs[1].x, t.cs[1].y), pair(t.cs[1].z, t.cs[1].w)};
+    const float si[8] = {t.sn[0].x, t.sn[0].y, t.sn[0].z, t.sn[0].w,
+                         t.sn[1].x, t.sn[1].y, t.sn[1].z, t.sn[1].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float s0 = a.sign * si[2 * i], s1 = a.sign * si[2 * i + 1];
+      const uint64_t lo = fma2(e.p[i], co[i], mul2(q.p[i], pair(-s0, -s1)));
+      q.p[i] = fma2(q.p[i], co[i], mul2(e.p[i], pair(s0, s1)));
+      e.p[i] = lo;
+    }
+    *reinterpret_cast<uint4*>(dst + t.c + a.half) = pack8<kBf16>(q);
+  }
+  *reinterpret_cast<uint4*>(dst + t.c) = pack8<kBf16>(e);
+}
+
+// The row at `src` transformed into `dst` by kLanes lanes (lane `gl`), V vectors
+// of 8 columns each.  `pos`: the row's rotation position, checked by the
+// caller.  src == dst is allowed: what a lane stores, no other lane reads,
+// but for the norm's pass, which the lanes' reduction ends.
+template <int V, bool kBf16, bool kWeighted>
+__device__ __forceinline__ void transform_row(const RowArgs& a, const uint16_t* src, uint16_t* dst,
+                                              int64_t pos, int gl, uint32_t mask) {
+  const int straight = a.dim - 2 * a.half;  // columns before the rotated ones
+  const int read = max(straight, a.norm_dim);
+  uint4 raw[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = (v * kLanes + gl) * 8;
+    raw[v] = make_uint4(0u, 0u, 0u, 0u);
+    if (c < read) raw[v] = *reinterpret_cast<const uint4*>(src + c);
+  }
+  Turn t;
+  t.c = -1;
+  if (a.half > 0) t = load_turn(a, src, pos, gl);
+  float scale = 1.0f;
+  if (a.norm_dim > 0) {
+    uint64_t sum2 = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = (v * G + gl) * 8;
-      raw[r][v] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows && c < a.dim)
-        raw[r][v] = *reinterpret_cast<const uint4*>(src + r * src_stride + c);
-    }
-  // The lane's rotated vector: columns rc .. rc + 7, -1 without one; by
-  // halves its partner is at columns pc.
-  int rc = -1, pc = 0;
+      if ((v * kLanes + gl) * 8 < a.norm_dim) {
+        const Eight e = unpack8<kBf16>(raw[v]);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int c = (v * G + gl) * 8;
-    if (a.half > 0 && c >= rot0 && c < a.dim) rc = c;
-  }
-  float4 cs[2], sn[2];
-  uint4 part[R];
-  const bool low = rc - rot0 < a.half;
-  if (rc >= 0) {
-    const int rel = rc - rot0;
-    if (a.interleaved) {
-      const size_t o = (size_t)pos * a.half + (rel >> 1);
-      cs[0] = __ldg(reinterpret_cast<const float4*>(a.cosv + o));
-      sn[0] = __ldg(reinterpret_cast<const float4*>(a.sinv + o));
-    } else {
-      pc = low ? rc + a.half : rc - a.half;
-      const size_t o = (size_t)pos * a.half + (low ? rel : rel - a.half);
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (r < rows) part[r] = *reinterpret_cast<const uint4*>(src + r * src_stride + pc);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        cs[i] = __ldg(reinterpret_cast<const float4*>(a.cosv + o) + i);
-        sn[i] = __ldg(reinterpret_cast<const float4*>(a.sinv + o) + i);
+        for (int i = 0; i < 4; ++i) sum2 = fma2(e.p[i], e.p[i], sum2);
       }
     }
-  }
-  float scale[R];
+    const float2 f = unpair(sum2);
+    float sum = f.x + f.y;
 #pragma unroll
-  for (int r = 0; r < R; ++r) scale[r] = 1.0f;
-  if (a.norm_dim > 0) {
-    float sum[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      sum[r] = 0.0f;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if ((v * G + gl) * 8 < a.norm_dim) {
-          float f[8];
-          unpack8<kBf16>(raw[r][v], f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum[r] += f[i] * f[i];
-        }
-      }
-    }
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1)
-#pragma unroll
-      for (int r = 0; r < R; ++r) sum[r] += __shfl_xor_sync(mask, sum[r], o);
-#pragma unroll
-    for (int r = 0; r < R; ++r) scale[r] = rsqrtf(sum[r] * a.inv_n + a.eps);
+    for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+    scale = rsqrtf(sum * a.inv_n + a.eps);
   }
   __syncwarp(mask);
-  // The rows stay packed: unpacked again below rather than kept as floats.
+  // The row stays packed: unpacked again below rather than kept as floats.
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      asm volatile("" : "+r"(raw[r][v].x), "+r"(raw[r][v].y), "+r"(raw[r][v].z), "+r"(raw[r][v].w));
+  for (int v = 0; v < V; ++v)
+    asm volatile("" : "+r"(raw[v].x), "+r"(raw[v].y), "+r"(raw[v].z), "+r"(raw[v].w));
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int c = (v * G + gl) * 8;
-    if (c >= a.dim) continue;
-    const bool normed = c < a.norm_dim, rotated = c == rc;
-    float w[8], wp[8];
-    const bool weighted = normed && a.weight != nullptr;
-    if (weighted) load_weight<kBf16>(a, c, w);
-    const bool partner = rotated && !a.interleaved;
-    const bool p_weighted = partner && pc < a.norm_dim && a.weight != nullptr;
-    if (p_weighted) load_weight<kBf16>(a, pc, wp);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (r >= rows) continue;
-      float f[8];
-      unpack8<kBf16>(raw[r][v], f);
-      if (normed) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= scale[r];
-      }
-      if (weighted) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= w[i];
-      }
-      if (rotated) {
-        if (a.interleaved) {
-          const float co[4] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w};
-          const float si[4] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float s = a.sign * si[i], x0 = f[2 * i], x1 = f[2 * i + 1];
-            f[2 * i] = x0 * co[i] - x1 * s;
-            f[2 * i + 1] = x1 * co[i] + x0 * s;
-          }
-        } else {
-          const float sg = low ? -a.sign : a.sign;
-          float p[8];
-          unpack8<kBf16>(part[r], p);
-          if (pc < a.norm_dim) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] *= scale[r];
-          }
-          if (p_weighted) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] *= wp[i];
-          }
-          const float co[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w,
-                               cs[1].x, cs[1].y, cs[1].z, cs[1].w};
-          const float si[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w,
-                               sn[1].x, sn[1].y, sn[1].z, sn[1].w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = f[i] * co[i] + p[i] * (sg * si[i]);
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + r * dst_stride + c) = pack8<kBf16>(f);
-    }
+    const int c = (v * kLanes + gl) * 8;
+    if (c < straight)
+      *reinterpret_cast<uint4*>(dst + c) =
+          pack8<kBf16>(norm8<kBf16, kWeighted>(a, raw[v], scale, c));
   }
+  store_turn<kBf16, kWeighted>(a, t, dst, scale);
+  for (int i = gl + kLanes; 4 * i < a.half; i += kLanes)
+    store_turn<kBf16, kWeighted>(a, load_turn(a, src, pos, i), dst, scale);
 }
 
 __device__ __forceinline__ void note_error(int32_t* err, int site, int detail, int extra) {
@@ -237,6 +249,11 @@ __device__ __forceinline__ void note_error(int32_t* err, int site, int detail, i
   }
 }
 
+// Lanes of this thread's row.
+__device__ __forceinline__ uint32_t row_mask() {
+  return ((1u << kLanes) - 1u) << (threadIdx.x & 31 & ~(kLanes - 1));
+}
+
 struct HeadArgs {
   const uint16_t* x;
   uint16_t* out;
@@ -244,36 +261,29 @@ struct HeadArgs {
   int32_t* err;
   int64_t x_t, x_h, o_t, o_h;
   int32_t heads;
-  int32_t chunks;  // of R heads a token
-  int32_t tasks;   // tokens * chunks
+  int32_t rows;
   bool pos64;
 };
 
-// Blocks an SM: registers for the rows in flight, 128 a thread for four rows of
-// up to 768 columns, 64 for one.
-template <int G, int V, int R, bool kBf16>
-__global__ void __launch_bounds__(kThreads, R == 1 ? 4 : V < 4 ? 2 : 1) norm_rope_kernel(RowArgs a, HeadArgs h) {
-  const int64_t task = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
-  if (task >= h.tasks) return;
-  const int gl = threadIdx.x & (G - 1);
-  const uint32_t mask = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (threadIdx.x & 31 & ~(G - 1));
-  const int t = (int)task / h.chunks, head = ((int)task - t * h.chunks) * R;
-  const int rows = min(R, h.heads - head);
-  int64_t pos = 0;
+template <int V, bool kBf16, bool kWeighted>
+__global__ void __launch_bounds__(kThreads, V <= 9 ? 3 : 2) norm_rope_kernel(RowArgs a, HeadArgs h) {
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  if (row >= h.rows) return;
+  const int gl = threadIdx.x & (kLanes - 1);
+  const int t = (int)row / h.heads, head = (int)row - t * h.heads;
   uint16_t* dst = h.out + t * h.o_t + head * h.o_h;
+  int64_t pos = 0;
   if (a.half > 0) {
     pos = h.pos64 ? __ldg(static_cast<const long long*>(h.positions) + t)
                   : (long long)__ldg(static_cast<const int32_t*>(h.positions) + t);
     if (pos < 0 || pos >= a.table_rows) {
       if (gl == 0) note_error(h.err, 52, t, head);
-      for (int r = 0; r < rows; ++r)
-        for (int c = gl * 8; c < a.dim; c += G * 8)
-          *reinterpret_cast<uint4*>(dst + r * h.o_h + c) = make_uint4(0u, 0u, 0u, 0u);
+      for (int c = gl * 8; c < a.dim; c += kLanes * 8)
+        *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
       return;
     }
   }
-  transform_rows<G, V, R, kBf16>(a, h.x + t * h.x_t + head * h.x_h, h.x_h, dst, h.o_h, rows, pos,
-                                 gl, mask);
+  transform_row<V, kBf16, kWeighted>(a, h.x + t * h.x_t + head * h.x_h, dst, pos, gl, row_mask());
 }
 
 struct AppendArgs {
@@ -286,18 +296,19 @@ struct AppendArgs {
   int32_t num_blocks, block_size, table_len, batch, total, ratio;
 };
 
-template <int G, int V, bool kBf16>
-__global__ void __launch_bounds__(kThreads, 4) append_norm_rope_kernel(RowArgs a, AppendArgs p) {
-  const int64_t row64 = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
+template <int V, bool kBf16, bool kWeighted>
+__global__ void __launch_bounds__(kThreads, V <= 9 ? 3 : 2)
+    append_norm_rope_kernel(RowArgs a, AppendArgs p) {
+  const int64_t row64 = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   if (row64 >= p.total) return;
   const int row = (int)row64;
-  const int gl = threadIdx.x & (G - 1);
-  const int shift = threadIdx.x & 31 & ~(G - 1);
-  const uint32_t mask = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << shift;
-  // The row's batch: the last b with cu[b] <= row, G probes a step.
+  const int gl = threadIdx.x & (kLanes - 1);
+  const uint32_t mask = row_mask();
+  // The row's batch: the last b with cu[b] <= row, kLanes probes
+  // a step.
   int lo = 0, hi = p.batch;
   while (lo < hi) {
-    const int step = (hi - lo + G) / G;
+    const int step = (hi - lo + kLanes) / kLanes;
     const int at = lo + gl * step;
     const bool le = at <= hi && __ldg(p.cu + at) <= row;
     const int n = __popc(__ballot_sync(mask, le));
@@ -321,10 +332,10 @@ __global__ void __launch_bounds__(kThreads, 4) append_norm_rope_kernel(RowArgs a
     if (gl == 0) note_error(p.err, 51, row, lo);
     return;
   }
-  transform_rows<G, V, 1, kBf16>(
-      a, p.rows + (size_t)row * a.dim, 0,
-      p.pool + ((size_t)blk * p.block_size + (size_t)(pos - lb * p.block_size)) * a.dim, 0, 1, rot,
-      gl, mask);
+  transform_row<V, kBf16, kWeighted>(
+      a, p.rows + (size_t)row * a.dim,
+      p.pool + ((size_t)blk * p.block_size + (size_t)(pos - lb * p.block_size)) * a.dim, rot, gl,
+      mask);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -362,44 +373,27 @@ int row_args(const SasRowTransform* tr, RowArgs* a) {
   return SAS_OK;
 }
 
-// Launches kernel<G, V, ..., bf16> over `tasks` groups, with the group and
-// the vectors a lane that hold a row of `dim` columns: the smallest G whose
-// lanes hold it at one vector each, else whole warps at up to 4 vectors.
-#define SAS_ROW_LAUNCH(G, KERNEL_BF16, KERNEL_FP16, ...)                                  \
-  do {                                                                                    \
-    const unsigned blocks = (unsigned)((tasks + kThreads / (G)-1) / (kThreads / (G)));    \
-    if (bf16)                                                                             \
-      KERNEL_BF16<<<blocks, kThreads, 0, stream>>>(__VA_ARGS__);                          \
-    else                                                                                  \
-      KERNEL_FP16<<<blocks, kThreads, 0, stream>>>(__VA_ARGS__);                          \
+// Calls LAUNCH(V, bf16, weighted) with the vectors a lane that hold a row.
+#define SAS_ROW_TYPES(V, LAUNCH)                                          \
+  do {                                                                    \
+    const bool weighted = a.weight != nullptr && a.norm_dim > 0;          \
+    if (bf16 && weighted) LAUNCH(V, true, true);                          \
+    else if (bf16) LAUNCH(V, true, false);                                \
+    else if (weighted) LAUNCH(V, false, true);                            \
+    else LAUNCH(V, false, false);                                         \
+  } while (0)
+#define SAS_ROW_DISPATCH(LAUNCH)                                          \
+  do {                                                                    \
+    if (a.dim <= 64) SAS_ROW_TYPES(1, LAUNCH);                            \
+    else if (a.dim <= 128) SAS_ROW_TYPES(2, LAUNCH);                      \
+    else if (a.dim <= 256) SAS_ROW_TYPES(4, LAUNCH);                      \
+    else if (a.dim <= 512) SAS_ROW_TYPES(8, LAUNCH);                      \
+    else if (a.dim <= 576) SAS_ROW_TYPES(9, LAUNCH);                      \
+    else SAS_ROW_TYPES(16, LAUNCH);                                       \
   } while (0)
 
-template <int R>
-void launch_heads(const RowArgs& a, const HeadArgs& h, bool bf16, cudaStream_t stream) {
-  const int64_t tasks = h.tasks;
-#define SAS_HEADS(G, V) \
-  SAS_ROW_LAUNCH(G, (norm_rope_kernel<G, V, R, true>), (norm_rope_kernel<G, V, R, false>), a, h)
-  if (a.dim <= 64) SAS_HEADS(8, 1);
-  else if (a.dim <= 128) SAS_HEADS(16, 1);
-  else if (a.dim <= 256) SAS_HEADS(32, 1);
-  else if (a.dim <= 512) SAS_HEADS(32, 2);
-  else if (a.dim <= 768) SAS_HEADS(32, 3);
-  else SAS_HEADS(32, 4);
-#undef SAS_HEADS
-}
-
-void launch_append(const RowArgs& a, const AppendArgs& p, bool bf16, cudaStream_t stream) {
-  const int64_t tasks = p.total;
-#define SAS_APPEND(G, V)                                                                    \
-  SAS_ROW_LAUNCH(G, (append_norm_rope_kernel<G, V, true>), (append_norm_rope_kernel<G, V, false>), \
-                 a, p)
-  if (a.dim <= 64) SAS_APPEND(8, 1);
-  else if (a.dim <= 128) SAS_APPEND(16, 1);
-  else if (a.dim <= 256) SAS_APPEND(32, 1);
-  else if (a.dim <= 512) SAS_APPEND(32, 2);
-  else if (a.dim <= 768) SAS_APPEND(32, 3);
-  else SAS_APPEND(32, 4);
-#undef SAS_APPEND
+unsigned blocks_of(int64_t rows) {
+  return (unsigned)((rows + kThreads / kLanes - 1) / (kThreads / kLanes));
 }
 
 }  // namespace
@@ -420,23 +414,15 @@ extern "C" int sas_norm_rope(const SasRowTransform* tr, const void* x, int64_t x
   if (!aligned16(x) || !aligned16(out) || (x_stride_token | x_stride_head | out_stride_token |
                                            out_stride_head) % 8 != 0)
     return SAS_ERR_INVALID;
-  // Four heads a group where that still leaves every SM sixteen warps or more;
-  // fewer rows are spread one a group for the shortest time.
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return SAS_ERR_CUDA;
-  const int per = heads >= 4 && rows / 4 >= 16 * (int64_t)sms ? 4 : 1;
-  const int chunks = (heads + per - 1) / per;
   const HeadArgs h{static_cast<const uint16_t*>(x), static_cast<uint16_t*>(out), positions, err,
-                   x_stride_token, x_stride_head, out_stride_token, out_stride_head, heads, chunks,
-                   tokens * chunks, positions_i64 != 0};
+                   x_stride_token, x_stride_head, out_stride_token, out_stride_head, heads,
+                   (int32_t)rows, positions_i64 != 0};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const bool bf16 = tr->dtype == SAS_DTYPE_BF16;
-  if (per == 4)
-    launch_heads<4>(a, h, bf16, stream);
-  else
-    launch_heads<1>(a, h, bf16, stream);
+#define SAS_HEADS(V, B, W) \
+  norm_rope_kernel<V, B, W><<<blocks_of(rows), kThreads, 0, stream>>>(a, h)
+  SAS_ROW_DISPATCH(SAS_HEADS);
+#undef SAS_HEADS
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
 
@@ -459,6 +445,10 @@ extern "C" int sas_kv_append_norm_rope(const SasRowTransform* tr, void* pool, in
                      block_table, cu_new, start_pos, err, num_blocks, block_size, table_len, batch,
                      total_new, cmp_ratio};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  launch_append(a, p, tr->dtype == SAS_DTYPE_BF16, stream);
+  const bool bf16 = tr->dtype == SAS_DTYPE_BF16;
+#define SAS_APPEND(V, B, W) \
+  append_norm_rope_kernel<V, B, W><<<blocks_of(total_new), kThreads, 0, stream>>>(a, p)
+  SAS_ROW_DISPATCH(SAS_APPEND);
+#undef SAS_APPEND
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
