@@ -200,23 +200,29 @@ __device__ __forceinline__ void store_turn(const RowArgs& a, const Turn& t, uint
   *reinterpret_cast<uint4*>(dst + t.c) = pack8<kBf16>(e);
 }
 
-// The row at `src` transformed into `dst` by kLanes lanes (lane `gl`), V vectors
-// of 8 columns each.  `pos`: the row's rotation position, checked by the
-// caller.  src == dst is allowed: what a lane stores, no other lane reads,
-// but for the norm's pass, which the lanes' reduction ends.
-template <int V, bool kBf16, Weights kW>
-__device__ __forceinline__ void transform_row(const RowArgs& a, const uint16_t* src, uint16_t* dst,
-                                              int64_t pos, int gl, uint32_t mask,
-                                              const float* sw) {
-  const int straight = a.dim - 2 * a.half;  // columns before the rotated ones
-  const int read = max(straight, a.norm_dim);
-  uint4 raw[V];
+// Columns of the row at `src` that lane `gl` norms or passes on.
+template <int V>
+__device__ __forceinline__ void load_row(const RowArgs& a, const uint16_t* src, int gl,
+                                         uint4 (&raw)[V]) {
+  const int read = max(a.dim - 2 * a.half, a.norm_dim);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int c = (v * kLanes + gl) * 8;
     raw[v] = make_uint4(0u, 0u, 0u, 0u);
     if (c < read) raw[v] = *reinterpret_cast<const uint4*>(src + c);
   }
+}
+
+// The row at `src`, of which load_row gave `raw`, transformed into `dst` by
+// kLanes lanes (lane `gl`), V vectors of 8 columns each.  `pos`: the row's
+// rotation position, checked by the caller.  src == dst is allowed: what a
+// lane stores, no other lane reads, but for the norm's pass, which the lanes'
+// reduction ends.
+template <int V, bool kBf16, Weights kW>
+__device__ __forceinline__ void transform_row(const RowArgs& a, uint4 (&raw)[V],
+                                              const uint16_t* src, uint16_t* dst, int64_t pos,
+                                              int gl, uint32_t mask, const float* sw) {
+  const int straight = a.dim - 2 * a.half;  // columns before the rotated ones
   Turn t;
   t.c = -1;
   if (a.half > 0) t = load_turn(a, src, pos, gl);
@@ -299,6 +305,9 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(RowArgs a, HeadA
   for (int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
        row < h.rows; row += step) {
     const int t = (int)row / h.heads, head = (int)row - t * h.heads;
+    const uint16_t* src = h.x + t * h.x_t + head * h.x_h;
+    uint4 raw[V];
+    load_row<V>(a, src, gl, raw);
     uint16_t* dst = h.out + t * h.o_t + head * h.o_h;
     int64_t pos = 0;
     if (a.half > 0) {
@@ -311,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(RowArgs a, HeadA
         continue;
       }
     }
-    transform_row<V, kBf16, kW>(a, h.x + t * h.x_t + head * h.x_h, dst, pos, gl, row_mask(), sw);
+    transform_row<V, kBf16, kW>(a, raw, src, dst, pos, gl, row_mask(), sw);
   }
 }
 
@@ -326,29 +335,36 @@ struct AppendArgs {
 };
 
 template <int V, bool kBf16, Weights kW>
-__global__ void __launch_bounds__(kThreads, V <= 9 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
     append_norm_rope_kernel(RowArgs a, AppendArgs p) {
   const int64_t row64 = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   if (row64 >= p.total) return;
   const int row = (int)row64;
   const int gl = threadIdx.x & (kLanes - 1);
   const uint32_t mask = row_mask();
-  // The row's batch: the last b with cu[b] <= row, kLanes probes
-  // a step.
-  int lo = 0, hi = p.batch;
-  while (lo < hi) {
+  // The row is on its way while its place is looked up.
+  const uint16_t* src = p.rows + (size_t)row * a.dim;
+  uint4 raw[V];
+  load_row<V>(a, src, gl, raw);
+  // The row's batch: the last b with cu[b] <= row, kLanes probes a step; the
+  // probes bring cu[b] and the batch's start along.
+  int lo = 0, hi = p.batch, first = 0, start = 0;
+  while (true) {
     const int step = (hi - lo + kLanes) / kLanes;
     const int at = lo + gl * step;
-    const bool le = at <= hi && __ldg(p.cu + at) <= row;
-    const int n = __popc(__ballot_sync(mask, le));
-    if (n == 0) break;
+    const int cu = at <= hi ? __ldg(p.cu + at) : 0;
+    const int st = at <= hi && at < p.batch ? __ldg(p.start + at) : 0;
+    const int n = __popc(__ballot_sync(mask, at <= hi && cu <= row));
+    if (n == 0) return;  // before the first sequence
+    first = __shfl_sync(mask, cu, n - 1, kLanes);
+    start = __shfl_sync(mask, st, n - 1, kLanes);
     lo += (n - 1) * step;
+    if (step == 1) break;
     hi = min(hi, lo + step - 1);
   }
-  const int first = __ldg(p.cu + lo);
-  // Rows before the first or behind the last sequence belong to none.
-  if (lo >= p.batch || row < first) return;
-  const int64_t pos = (int64_t)__ldg(p.start + lo) + (row - first);
+  // Rows behind the last sequence belong to none.
+  if (lo >= p.batch) return;
+  const int64_t pos = (int64_t)start + (row - first);
   const int64_t lb = pos >= 0 ? pos / p.block_size : -1;
   const int blk =
       (lb >= 0 && lb < p.table_len) ? __ldg(p.table + (size_t)lo * p.table_len + lb) : -1;
@@ -362,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, V <= 9 ? 3 : 2)
     return;
   }
   transform_row<V, kBf16, kW>(
-      a, p.rows + (size_t)row * a.dim,
+      a, raw, src,
       p.pool + ((size_t)blk * p.block_size + (size_t)(pos - lb * p.block_size)) * a.dim, rot, gl,
       mask, nullptr);
 }
