@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdlib>
 #include <cstring>
 #include <vector>
@@ -40,10 +41,8 @@ WorkspaceLayout layout_for(const SasPlanInfo& info, int32_t num_heads, int32_t h
 
 int resolve_sms(int32_t requested) {
   if (requested > 0) return requested;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return sms;
+  int dev = 0;
+  return sas::current_device_sms(&dev);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -70,6 +69,22 @@ int validate(const SasProblem& p, const SasFwdParams& f) {
 }
 
 }  // namespace
+
+namespace sas {
+
+int current_device_sms(int* device) {
+  static std::atomic<int> known[kMaxDevices];  // 0: not asked yet
+  if (cudaGetDevice(device) != cudaSuccess || *device < 0 || *device >= kMaxDevices) return 0;
+  int sms = known[*device].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, *device) != cudaSuccess)
+      return 0;
+    known[*device].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
+}
+
+}  // namespace sas
 
 extern "C" int sas_fwd_workspace_size(const SasProblem* prob, int32_t num_sms, size_t* bytes) {
   if (!prob || !bytes) return SAS_ERR_INVALID;

@@ -42,6 +42,8 @@
 #include <math_constants.h>
 #include <stddef.h>
 
+#include <atomic>
+
 #include "sas_dev.cuh"
 
 namespace sas {
@@ -680,12 +682,15 @@ bool ix_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t mid, uint6
 }
 
 template <int kChunks, int kHp>
-int ix_launch(const IxArgs& a, int grid, const CUtensorMap& q, const CUtensorMap& k,
+int ix_launch(const IxArgs& a, int grid, int dev, const CUtensorMap& q, const CUtensorMap& k,
               cudaStream_t stream) {
-  // Per device, so set on every call (well under a microsecond).
-  if (cudaFuncSetAttribute(index_scores_kernel<kChunks, kHp>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize, kIxSmem) != cudaSuccess)
-    return SAS_ERR_CUDA;
+  static std::atomic<bool> configured[kMaxDevices];
+  if (!configured[dev].load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(index_scores_kernel<kChunks, kHp>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, kIxSmem) != cudaSuccess)
+      return SAS_ERR_CUDA;
+    configured[dev].store(true, std::memory_order_relaxed);
+  }
   index_scores_kernel<kChunks, kHp><<<grid, kIxThreads, kIxSmem, stream>>>(a, q, k);
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
@@ -715,10 +720,9 @@ extern "C" int sas_index_scores(const SasIndexParams* params, void* stream_ptr) 
   if (((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.key_pool)) & 15) != 0)
     return SAS_ERR_INVALID;
   using namespace sas;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return SAS_ERR_CUDA;
+  int dev = 0;
+  const int sms = current_device_sms(&dev);
+  if (sms <= 0) return SAS_ERR_CUDA;
 
   IxArgs a{};
   a.p = p;
@@ -766,10 +770,10 @@ extern "C" int sas_index_scores(const SasIndexParams* params, void* stream_ptr) 
   const int grid = 2 * (int)(items < pairs ? items : pairs);
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
 #define SAS_IX(C)                                                       \
-  (hp == 16   ? ix_launch<C, 16>(a, grid, tm_q, tm_k, stream)           \
-   : hp == 32 ? ix_launch<C, 32>(a, grid, tm_q, tm_k, stream)           \
-   : hp == 64 ? ix_launch<C, 64>(a, grid, tm_q, tm_k, stream)           \
-              : ix_launch<C, 128>(a, grid, tm_q, tm_k, stream))
+  (hp == 16   ? ix_launch<C, 16>(a, grid, dev, tm_q, tm_k, stream)           \
+   : hp == 32 ? ix_launch<C, 32>(a, grid, dev, tm_q, tm_k, stream)           \
+   : hp == 64 ? ix_launch<C, 64>(a, grid, dev, tm_q, tm_k, stream)           \
+              : ix_launch<C, 128>(a, grid, dev, tm_q, tm_k, stream))
   return p.head_dim > 64 ? SAS_IX(2) : SAS_IX(1);
 #undef SAS_IX
 }

@@ -42,6 +42,10 @@ struct FwdArgs {
   int32_t slot_dump_cap;
 };
 
+// SMs of the current device, whose number goes to *device; 0 if there is none.
+constexpr int kMaxDevices = 64;
+int current_device_sms(int* device);
+
 int launch_fwd(const FwdArgs& args, int grid, cudaStream_t stream);
 int launch_fwd_pair(const FwdArgs& args, int workers, cudaStream_t stream);
 

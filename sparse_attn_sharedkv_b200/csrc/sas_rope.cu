@@ -24,6 +24,7 @@
 #include <stdint.h>
 
 #include "sas.h"
+#include "sas_kernels.h"
 
 namespace {
 
@@ -465,10 +466,9 @@ extern "C" int sas_norm_rope(const SasRowTransform* tr, const void* x, int64_t x
                    (int32_t)rows, positions_i64 != 0};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const bool bf16 = tr->dtype == SAS_DTYPE_BF16;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return SAS_ERR_CUDA;
+  int dev = 0;
+  const int sms = sas::current_device_sms(&dev);
+  if (sms <= 0) return SAS_ERR_CUDA;
   const unsigned blocks = blocks_of(rows), full = 2u * (unsigned)sms;
 #define SAS_HEADS(V, B, W) norm_rope_kernel<V, B, W><<<grid, kThreads, 0, stream>>>(a, h)
   if (blocks > full) {

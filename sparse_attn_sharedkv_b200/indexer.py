@@ -133,11 +133,14 @@ def index_scores(q: torch.Tensor, weights: torch.Tensor, *, key_pool: torch.Tens
                                cmp_ratio, layout_q, max_keys)
     dev, total = q.device, p.total_tokens
     # Rows of whole 16-byte vectors.
-    scores = torch.empty((total, (N + 3) // 4 * 4), dtype=torch.float32, device=dev)[:, :N]
+    stride = (N + 3) // 4 * 4
+    scores = weights.new_empty((total, stride))
+    if stride != N:
+        scores = scores[:, :N]
     lengths = torch.empty(total, dtype=torch.int32, device=dev) if return_lengths else None
     if total > 0:
         err = torch.zeros(4, dtype=torch.int32, device=dev) if _check_device_errors() else None
-        p.scores, p.score_stride = scores.data_ptr(), scores.stride(0)
+        p.scores, p.score_stride = scores.data_ptr(), stride
         p.lengths = lengths.data_ptr() if lengths is not None else None
         p.err = err.data_ptr() if err is not None else None
         p.first_token, p.num_tokens, p.fill = 0, total, 1
@@ -174,7 +177,7 @@ def select_topk(scores: torch.Tensor, topk: int, *,
     rows = shape[0] if len(shape) == 2 else shape[0] * shape[1]
     if rows > (2 ** 31 - 1) // 8:
         raise ValueError("scores hold more than 2^28 - 1 rows")
-    out = torch.empty((*shape[:-1], 1, topk), dtype=torch.int32, device=dev)
+    out = scores.new_empty((*shape[:-1], 1, topk), dtype=torch.int32)
     if lengths is not None:
         if lengths.numel() != rows:
             raise ValueError("lengths must have one entry per row of scores")

@@ -141,7 +141,7 @@ def norm_rope(x: torch.Tensor, positions: Optional[torch.Tensor] = None,
             positions = positions.to(dev).contiguous()
         pos_ptr, pos64 = positions.data_ptr(), positions.dtype is torch.int64
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
         o = (out.data_ptr(), H * D, D)
     else:
         if out.shape != shape or out.dtype != x.dtype or out.device != dev:
