@@ -11,27 +11,28 @@
 //
 // Work.  A group is up to 256 / Hp consecutive tokens of one sequence (Hp:
 // the heads, padded to 16, 32, 64 or 128), so that the (token, head) pairs of
-// a group are the N <= 256 columns of one MMA; its M = 256 rows are a tile of
-// 256 keys, 128 in each CTA of a pair (tcgen05.mma.cta_group::2).  With keys
-// in the rows, a thread of the epilogue owns one key and sums over heads along
-// its own TMEM lane, without exchanging anything; the weights of its columns
-// stay in registers over all the key tiles of a group.  The pair halves what
-// the queries take of each SM's shared memory (room for five key stages beside
-// two query buffers) and the operand reads of each MMA.  An item is a group
-// and a span of its key tiles; a persistent pair takes every num_pairs-th
-// item.  Tiles that no token of the group sees are filled with -inf without
-// loads.
+// a group are up to 256 columns, in two halves of whole tokens; the rows are a
+// tile of 256 keys, 128 in each CTA of a pair, and a half is one
+// tcgen05.mma.cta_group::2 of M = 256, N = 128 a step of 16 dims.  With keys in
+// the rows, a thread of the epilogue owns one key and sums over heads along
+// its own TMEM lane, without exchanging anything; the weights of its half's
+// columns stay in registers over all the key tiles of a group.  The pair
+// halves what the queries take of each SM's shared memory, which leaves room
+// for five key stages beside two query buffers.  Each half has two
+// accumulators of its own, so that the two epilogue warpgroups do not wait for
+// each other.  An item is a group and a span of its key tiles; a persistent
+// pair takes every num_pairs-th item.  Tiles that no token of the group sees
+// are filled with -inf without loads.
 //
 // Warp roles in each CTA (384 threads, one CTA per SM):
 //   0, 3   keys, every other tile each: page lookup, TMA into a ring of stages
 //          (boxes of a page's rows where the page size allows, tile::gather4
 //          else)
-//   1      CTA 0: MMA issue (one lane), accumulators alternating between two
-//          halves of TMEM
+//   1      CTA 0: MMA issue (one elected lane)
 //   2      items: the group of the next item, its queries into the other of
 //          two buffers, its weights; the -inf fill; TMEM
-//   4-11   epilogue: warpgroup g takes columns 128 g .. 128 g + 127 of each
-//          accumulator: relu, weight, sum over heads, mask, store
+//   4-11   epilogue: warpgroup g takes half g: relu, weight, sum over heads,
+//          mask, store
 //
 // TMA loads of both CTAs complete on the leader's barriers; the leader's
 // commits arrive in both CTAs; CTA 1's epilogue releases accumulators on the
@@ -53,12 +54,13 @@ constexpr int kIxThreads = 384;
 constexpr int kIxKeys = 128;               // keys of a CTA's tile
 constexpr int kIxTile = 2 * kIxKeys;       // keys of the pair's tile (M)
 constexpr int kIxCols = 256;               // (token, head) columns of a group (N)
-constexpr int kIxHalf = kIxCols / 2;       // columns of an epilogue warpgroup
+constexpr int kIxHalf = kIxCols / 2;       // columns of half a group
 constexpr int kIxTokens = kIxCols / 16;    // tokens of a group at most
 constexpr int kIxMaxStages = 8;
 constexpr int kIxBits = 16;                // tiles whose page bits are kept
 constexpr int kIxItems = 4;                // items described ahead
-constexpr int kIxQChunk = kIxHalf * 128;   // 64 dims of a CTA's half of the columns
+constexpr int kIxQHalf = kIxHalf / 2 * 128;  // 64 dims of a CTA's columns of one half
+constexpr int kIxQChunk = 2 * kIxQHalf;
 constexpr int kIxKChunk = kIxKeys * 128;   // 64 dims of a CTA's key tile
 constexpr int kIxSmem = 232448;            // the per-block opt-in maximum
 
@@ -76,7 +78,8 @@ struct IxInfo {
 struct IxCtl {
   uint64_t q_full[2], q_empty[2];  // full: leader, one arrival per CTA and the bytes of both
   uint64_t k_full[kIxMaxStages], k_empty[kIxMaxStages];
-  uint64_t acc_full[2], acc_empty[2];  // empty: leader, the epilogue warps of both CTAs
+  // [half][buffer]; empty: leader, the half's epilogue warps of both CTAs.
+  uint64_t acc_full[2][2], acc_empty[2][2];
   uint64_t item_full[kIxItems], item_empty[kIxItems];
   uint64_t w_full, w_empty;
   uint64_t bits_full[kIxBits];
@@ -86,8 +89,9 @@ struct IxCtl {
   uint8_t issued[kIxMaxStages];  // 1 + parity of the stage's last load, 0 before the first
   // Bit r of byte i of a tile: key 8 i + r has a page.  The slot of tile n is
   // written again for tile n + kIxBits, after the MMAs of tile n + kIxBits -
-  // stages, whose accumulator the epilogue released behind tile n + kIxBits -
-  // stages - 3 >= n.
+  // stages, whose accumulators the epilogue released behind tile n + kIxBits -
+  // stages - 3 >= n (a half without tokens in an item has released all of its
+  // before that item's first MMA).
   uint8_t bits[kIxBits][16];
   IxInfo items[kIxItems];
   alignas(16) float w[kIxCols];  // read as 16-byte vectors
@@ -186,6 +190,17 @@ __device__ __forceinline__ float relu_nan(uint32_t bits) {
   float y;
   asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(__uint_as_float(bits)));
   return y;
+}
+
+// One lane of a converged warp: the code behind it runs once, and the compiler
+// keeps the descriptors of the MMAs there in uniform registers (behind lane ==
+// 0 it copies them lane by lane: 120 cycles an MMA against 30).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
 }
 
 // Pairs of fp32 in one 64-bit register, for the packed FMA.
@@ -361,12 +376,12 @@ __device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_
   constexpr int kTok = kIxHalf / kHp;  // tokens of a warpgroup
   const int tid = threadIdx.x - 128, wg = tid >> 7, lane = tid & 31;
   const int row = tid & 127;
-  const uint32_t base = tmem + ((uint32_t)(row & ~31) << 16) + (uint32_t)(wg * kIxHalf);
-  const uint32_t empty0 = peer_addr(smem_addr(&ctl.acc_empty[0]), 0);
+  const uint32_t base = tmem + ((uint32_t)(row & ~31) << 16) + (uint32_t)(wg * 2 * kIxHalf);
+  const uint32_t empty0 = peer_addr(smem_addr(&ctl.acc_empty[wg][0]), 0);
   uint64_t w[kIxHalf / 2];
 #pragma unroll
   for (int i = 0; i < kIxHalf / 2; ++i) w[i] = 0;
-  int n = 0, m = 0;
+  int n = 0, u = 0, m = 0;  // tiles of the pair, of this half, items with tiles
   for (int i = 0; i < count; ++i) {
     const IxInfo* info = ix_next(ctl, i, p.err, 73);
     if (info == nullptr) return;
@@ -388,18 +403,22 @@ __device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_addr(&ctl.w_empty));
     ++m;
-    float* out = p.scores + (size_t)max(tok0, 0) * p.score_stride;
-    for (int t = t0; t < tc; ++t, ++n) {
-      const int b = n & 1, slot = n % kIxBits;
-      if (!ix_wait(ctl, &ctl.acc_full[b], (n >> 1) & 1, p.err, 80) ||
+    if (live <= 0) {
+      n += tc - t0;
+      continue;
+    }
+    float* out = p.scores + (size_t)tok0 * p.score_stride;
+    for (int t = t0; t < tc; ++t, ++n, ++u) {
+      const int b = u & 1, slot = n % kIxBits;
+      if (!ix_wait(ctl, &ctl.acc_full[wg][b], (u >> 1) & 1, p.err, 80) ||
           !ix_wait(ctl, &ctl.bits_full[slot], (n / kIxBits) & 1, p.err, 81))
         return;
       tc_fence_after();
       const int key = t * kIxTile + rank * kIxKeys + row;
       const bool paged = (ctl.bits[slot][row >> 3] >> (row & 7)) & 1;
-      const uint32_t acc = base + (uint32_t)(b * kIxCols);
+      const uint32_t acc = base + (uint32_t)(b * kIxHalf);
       uint32_t v[2][16];
-      if (live > 0) tmem_ld16(acc, v[0]);
+      tmem_ld16(acc, v[0]);
       uint64_t s0 = 0, s1 = 0;
 #pragma unroll
       for (int c = 0; c < kIxHalf / 16; ++c) {
@@ -407,8 +426,13 @@ __device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_
         const int tok = c / kPieces;
         if (tok < live) {
           tmem_wait_ld();
-          if (c + 1 < kIxHalf / 16 && (c + 1) / kPieces < live)
+          if (c + 1 < kIxHalf / 16 && (c + 1) / kPieces < live) {
             tmem_ld16(acc + 16u * (c + 1), v[(c + 1) & 1]);
+          } else {  // all read: the accumulator is free
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_remote(empty0 + 8u * (uint32_t)b);
+          }
 #pragma unroll
           for (int k = 0; k < 16; k += 4) {
             const uint32_t* x = &v[c & 1][k];
@@ -423,9 +447,6 @@ __device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_remote(empty0 + 8u * (uint32_t)b);
     }
   }
 }
@@ -472,18 +493,22 @@ __device__ __forceinline__ void ix_items(const IxArgs& a, IxCtl& ctl, uint32_t s
     if (busy) {
       const int qb = m & 1;
       if (!ix_wait(ctl, &ctl.q_empty[qb], ((m >> 1) & 1) ^ 1, p.err, 72)) break;
-      // Each CTA holds the columns of half of the tokens.
-      const int half = (r.live + 1) >> 1;
-      const int mine = rank == 0 ? half : r.live - half;
+      // Half g holds the tokens g kTok ..; of its columns each CTA holds half,
+      // in units of half a token's heads.
+      constexpr int kTok = kIxHalf / kHp, kUnit = kHp / 2;
       const uint32_t bar = full0 + 8u * (uint32_t)qb;
-      if (lane == 0) arrive_tx_cluster(bar, (uint32_t)(mine * kChunks * kHp * 128), false);
+      if (lane == 0) arrive_tx_cluster(bar, (uint32_t)(r.live * kChunks * kUnit * 128), false);
       __syncwarp();
-      if (lane < mine) {
+      const int g = lane / kTok, u = lane % kTok;  // unit u of half g
+      const int tokens = min(kTok, r.live - g * kTok);
+      if (g < 2 && u < tokens) {
+        const int unit = rank * tokens + u;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
-          tma_load_3d_pair(
-              sQ + (uint32_t)(qb * IxSmem<kChunks>::kQ + c * kIxQChunk + lane * kHp * 128), tm_q,
-              c * 64, 0, p.first_token + r.tok0 + rank * half + lane, bar);
+          tma_load_3d_pair(sQ + (uint32_t)(qb * IxSmem<kChunks>::kQ + c * kIxQChunk +
+                                           g * kIxQHalf + u * kUnit * 128),
+                           tm_q, c * 64, (unit & 1) * kUnit,
+                           p.first_token + r.tok0 + g * kTok + (unit >> 1), bar);
       }
       if (!ix_wait(ctl, &ctl.w_empty, (m & 1) ^ 1, p.err, 78)) break;
 #pragma unroll
@@ -519,53 +544,71 @@ __device__ __forceinline__ void ix_issue(const IxArgs& a, IxCtl& ctl, uint32_t s
                                          uint32_t tmem, int count, int rank, int lane) {
   using L = IxSmem<kChunks>;
   const SasIndexParams& p = a.p;
-  int s = 0, ph = 0, b = 0, bph = 1;  // key stage, accumulator and the parities awaited
+  constexpr int kTok = kIxHalf / kHp;
+  int s = 0, ph = 0;        // key stage and the parity awaited
+  int units[2] = {0, 0};    // accumulators filled of each half
   int m = 0;
   const int steps = (p.head_dim + 15) / 16;
-  bool ok = true;
-  for (int i = 0; ok && i < count; ++i) {
+  for (int i = 0; i < count; ++i) {
     const IxInfo* info = ix_next(ctl, i, p.err, 67);
     if (info == nullptr) break;
-    const int t0 = info->t0, tc = info->tc;
-    const int cols = ((info->live + 1) & ~1) * kHp;
+    const int t0 = __shfl_sync(0xffffffffu, info->t0, 0);
+    const int tc = __shfl_sync(0xffffffffu, info->tc, 0);
+    const int live = __shfl_sync(0xffffffffu, info->live, 0);
     ix_done(ctl, i, lane);
     if (rank != 0 || tc == t0) continue;
-    if (lane == 0) {
-      const int qb = m & 1;
-      const uint32_t idesc = a.idesc | (uint32_t)(cols >> 3) << 17;
-      const uint64_t dq = smem_desc(sQ + (uint32_t)(qb * L::kQ), 16, 1024);
-      ok = wait_bar(&ctl, &ctl.q_full[qb], (uint32_t)(m >> 1) & 1, p.err, 74);
-      for (int t = t0; ok && t < tc; ++t) {
-        ok = wait_bar(&ctl, &ctl.k_full[s], (uint32_t)ph, p.err, 75) &&
-             wait_bar(&ctl, &ctl.acc_empty[b], (uint32_t)bph, p.err, 76);
+    const int halves = live > kTok ? 2 : 1;
+    bool ok = true;
+    // A half that this item leaves out is done with the items before: its
+    // epilogue still reads the page bits of their tiles.
+    if (halves == 1)
+      for (int u = max(0, units[1] - 2); ok && u < units[1]; ++u)
+        ok = ix_wait(ctl, &ctl.acc_empty[1][u & 1], (u >> 1) & 1, p.err, 77);
+    const int qb = m & 1;
+    ++m;
+    const uint64_t dq0 = smem_desc(sQ + (uint32_t)(qb * L::kQ), 16, 1024);
+    ok = ok && ix_wait(ctl, &ctl.q_full[qb], ((m - 1) >> 1) & 1, p.err, 74);
+    for (int t = t0; ok && t < tc; ++t) {
+      ok = ix_wait(ctl, &ctl.k_full[s], ph, p.err, 75);
+      const uint64_t dk = smem_desc(sK + (uint32_t)(s * kChunks * kIxKChunk), 16, 1024);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (!ok || g >= halves) break;
+        const int b = units[g] & 1;
+        ok = ix_wait(ctl, &ctl.acc_empty[g][b], ((units[g] >> 1) & 1) ^ 1, p.err, 76);
         if (!ok) break;
         tc_fence_after();
-        const uint64_t dk = smem_desc(sK + (uint32_t)(s * kChunks * kIxKChunk), 16, 1024);
-        const uint32_t acc = tmem + (uint32_t)(b * kIxCols);
+        const uint32_t cols = (uint32_t)(min(kTok, live - g * kTok) * kHp);
+        const uint32_t idesc = a.idesc | (cols >> 3) << 17;
+        const uint64_t dq = dq0 + (uint64_t)(g * kIxQHalf >> 4);
+        const uint32_t acc = tmem + (uint32_t)((2 * g + b) * kIxHalf);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 4 * kChunks; ++k) {
-          const uint32_t in = (uint32_t)(k & 3) * 32u, ch = (uint32_t)(k >> 2);
-          if (k < steps)
-            mma2(acc, dk + ((in + ch * kIxKChunk) >> 4), dq + ((in + ch * kIxQChunk) >> 4), idesc,
-                 k > 0);
+          for (int k = 0; k < 4 * kChunks; ++k) {
+            const uint32_t in = (uint32_t)(k & 3) * 32u, ch = (uint32_t)(k >> 2);
+            if (k < steps)
+              mma2(acc, dk + ((in + ch * kIxKChunk) >> 4), dq + ((in + ch * kIxQChunk) >> 4),
+                   idesc, k > 0);
+          }
+          commit_both(smem_addr(&ctl.acc_full[g][b]));
+          if (g + 1 == halves) commit_both(smem_addr(&ctl.k_empty[s]));
         }
-        commit_both(smem_addr(&ctl.k_empty[s]));
-        commit_both(smem_addr(&ctl.acc_full[b]));
-        if (++s == L::kStages) {
-          s = 0;
-          ph ^= 1;
-        }
-        b ^= 1;
-        bph ^= b ^ 1;
+        __syncwarp();
+        ++units[g];
       }
-      commit_both(smem_addr(&ctl.q_empty[qb]));
+      if (++s == L::kStages) {
+        s = 0;
+        ph ^= 1;
+      }
     }
-    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-    ++m;
+    if (!ok) break;
+    if (elect_one()) commit_both(smem_addr(&ctl.q_empty[qb]));
+    __syncwarp();
   }
   // Every MMA has read its operands before either CTA goes.
-  if (rank == 0 && lane == 0) {
-    commit_both(smem_addr(&ctl.drain));
+  if (rank == 0) {
+    if (elect_one()) commit_both(smem_addr(&ctl.drain));
+    __syncwarp();
     ix_settle(&ctl.drain, 0u);
   }
 }
@@ -588,8 +631,10 @@ __global__ void __launch_bounds__(kIxThreads, 1) __cluster_dims__(2, 1, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_addr(&ctl.q_full[i]), 2);
       mbar_init(smem_addr(&ctl.q_empty[i]), 1);
-      mbar_init(smem_addr(&ctl.acc_full[i]), 1);
-      mbar_init(smem_addr(&ctl.acc_empty[i]), 16);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(smem_addr(&ctl.acc_full[i][b]), 1);
+        mbar_init(smem_addr(&ctl.acc_empty[i][b]), 8);
+      }
     }
     for (int i = 0; i < kIxMaxStages; ++i) {
       mbar_init(smem_addr(&ctl.k_full[i]), 2);
@@ -754,7 +799,7 @@ extern "C" int sas_index_scores(const SasIndexParams* params, void* stream_ptr) 
 
   alignas(64) CUtensorMap tm_q, tm_k;
   const uint64_t D = (uint64_t)p.head_dim, H = (uint64_t)p.num_heads, T = (uint64_t)p.total_tokens;
-  if (!ix_map(&tm_q, p.q, D, H, T, (uint32_t)hp, true)) return SAS_ERR_CUDA;
+  if (!ix_map(&tm_q, p.q, D, H, T, (uint32_t)hp / 2, true)) return SAS_ERR_CUDA;
   if (a.no_row > 0) {
     if (!ix_map(&tm_k, p.key_pool, D, (uint64_t)a.no_row, 1, (uint32_t)box, false))
       return SAS_ERR_CUDA;
