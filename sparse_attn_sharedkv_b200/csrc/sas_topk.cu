@@ -13,13 +13,16 @@
 //      scores spread (a bin then holds a few, and the shared-memory atomics
 //      seldom meet); the bin in which the K-th largest lies.  The bin is the
 //      low bits of a float near 2^23, so no conversion is needed;
-//   3. if that bin holds more than 128, once more inside of it;
-//   4. the scores of the last bin are listed and ranked by (score, position):
-//      the K-th is the threshold;
-//   5. the positions at or above the threshold are counted and written.
+//   3. scores in higher bins are selected, those of the border bin listed (if
+//      they are more than 512, those of one bin of a second histogram inside
+//      of it);
+//   4. among more than 32 listed, a histogram inside of the bin again; the
+//      border ones left are ranked by (score, position), and the list's
+//      winners are marked for the threads that hold them;
+//   5. the selected positions are counted and written.
 //
-// Any other row (infinities, NaN, a single value, more than 128 left after
-// step 3) is read again as unsigned keys of the same order: histograms linear
+// Any other row (infinities, NaN, a single value, more left than the lists
+// hold) is read again as unsigned keys of the same order: histograms linear
 // in the keys divide the range of the border keys by at least 512 a round
 // until 128 or a single key are left; equal keys are taken by a count over
 // their positions.
@@ -38,6 +41,7 @@
 namespace {
 
 constexpr int kBins = 1024;
+constexpr int kCand = 512;                 // border scores listed
 constexpr int kList = 128;                 // keys ranked directly
 constexpr int kPer = 16;                   // keys of a thread
 constexpr uint32_t kNegInf = 0x007fffffu;  // key of -inf
@@ -96,9 +100,11 @@ struct TopkShared {
   uint32_t wmin[T / 32], wmax[T / 32], wcnt[T / 32], wsum[T / 32];
   uint32_t rmin[C], rmax[C], rcnt[C], rtot[C];  // one entry per block of the cluster
   uint32_t bin, above, inside;                  // found in the histogram, bin from the top
-  uint32_t listed;
-  uint32_t list_key[kList], list_pos[kList];  // of the cluster, in block 0
-  uint32_t key[kList], pos[kList];            // own copy
+  uint32_t listed, ranked;
+  uint32_t list_key[kCand], list_pos[kCand];            // of the cluster, in block 0
+  uint32_t mine_key[C > 1 ? kCand : 1], mine_pos[C > 1 ? kCand : 1];  // own copy
+  uint32_t key[kList], pos[kList];
+  uint32_t taken[T];  // listed scores of each thread that are selected
   uint32_t thr_key, thr_pos;
 };
 
@@ -137,17 +143,18 @@ __device__ __forceinline__ void row_reduce(TopkShared<T, C>& s, int rank, uint32
 // The bin of the histograms (of all the row's blocks) in which the need-th
 // largest lies: into s.bin, with the count above it and the one inside.
 // Starts and ends with a barrier of the row / the block.
-template <int T, int C>
+// kAlone: the histogram of this block alone.
+template <int T, int C, bool kAlone = C == 1>
 __device__ __forceinline__ void find_bin(TopkShared<T, C>& s, uint32_t need) {
   constexpr int W = T / 32, kOwn = kBins / T;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  row_sync<C>();
+  row_sync<kAlone ? 1 : C>();
   uint32_t h[kOwn], sum = 0;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     const int b = tid * kOwn + i;
     h[i] = 0;
-    if constexpr (C == 1) {
+    if constexpr (kAlone) {
       h[i] = s.hist[b];
     } else {
 #pragma unroll
@@ -180,16 +187,18 @@ __device__ __forceinline__ void find_bin(TopkShared<T, C>& s, uint32_t need) {
 }
 
 // Count, over the row's positions, of the flags (bit i: the thread's key of
-// round i) before each of the thread's keys: at[i] for round i.  Returns the
+// round i, none behind round `last`) before each of the thread's keys: at[i] for round i.  Returns the
 // block's total and, in *block_base, the count in the blocks before it.
 template <int T, int C>
 __device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, uint32_t flags,
-                                                 uint32_t (&at)[kPer], uint32_t* block_base) {
+                                                 int last, uint32_t (&at)[kPer],
+                                                 uint32_t* block_base) {
   constexpr int W = T / 32, kChunk = W / 2;  // kPer * W counts: kChunk of them a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t incl4[kPer / 4];
+  uint32_t incl4[kPer / 4] = {};
 #pragma unroll
   for (int g = 0; g < kPer / 4; ++g) {
+    if (4 * g > last) break;
     // Bits 0 .. 3 of the group into the low bits of four bytes.
     const uint32_t own = ((flags >> (4 * g) & 15u) * 0x00204081u) & 0x01010101u;
     uint32_t v = own;  // at most 32 in each byte
@@ -225,8 +234,10 @@ __device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, 
   }
   const uint32_t start = incl - sum + part;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
+  for (int i = 0; i < kPer; ++i) {
+    if (i > last) break;
     at[i] += __shfl_sync(0xffffffffu, start, 2 * i + (warp >= kChunk ? 1 : 0));
+  }
   const uint32_t total = __shfl_sync(0xffffffffu, incl, 31);
   *block_base = 0;
   if constexpr (C > 1) {
@@ -339,7 +350,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
     } else if (equal) {
       // The first `need` of the equal keys by position.
       uint32_t at[kPer], base;
-      count_before<T, C>(s, rank, cand, at, &base);
+      count_before<T, C>(s, rank, cand, kPer - 1, at, &base);
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         if (cand >> i & 1) sel |= (base + at[i] < need ? 1u : 0u) << i;
@@ -438,22 +449,27 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
     for (int i = rank * T + tid; i < K; i += C * T) o[i] = -1;
     return;
   }
-  // The block's part of the row; rounds in which the thread holds a score.
+  // The block's part of the row; the thread holds a score in `rounds` rounds,
+  // some thread does up to round `last`.
   const int part = (n + C - 1) / C;
   const int begin = min(n, rank * part), end = min(n, begin + part);
-  const int rounds = (end - begin - tid + T - 1) / T;
+  const int rounds = (end - begin - tid + T - 1) / T, last = (end - begin - 1) / T;
 
   // Empty places hold the row's first score, which changes no extremum.
   const float first = __ldg(x);
   float v[kPer];
+  float low = first, high = first;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) v[i] = i < rounds ? __ldg(x + begin + i * T + tid) : first;
+  for (int i = 0; i < kPer; ++i) {
+    if (i > last) break;
+    v[i] = i < rounds ? __ldg(x + begin + i * T + tid) : first;
+  }
   for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
-  if (tid == 0) s.listed = 0;
-
-  float low = v[0], high = v[0];
+  s.taken[tid] = 0;
+  if (tid == 0) s.listed = s.ranked = 0;
 #pragma unroll
-  for (int i = 1; i < kPer; ++i) {
+  for (int i = 0; i < kPer; ++i) {
+    if (i > last) break;
     low = min_nan(low, v[i]);
     high = max_nan(high, v[i]);
   }
@@ -476,9 +492,9 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
     high = warp_max(__uint_as_float(s.rmax[lane % C]));
   }
 
-  uint32_t sel = 0, able = (uint32_t)n;
+  uint32_t sel = 0, able = (uint32_t)n;  // bit i of sel: v[i] is selected
   const float scale = __fdividef((float)(kBins - 2), high - low);
-  bool general = false;
+  bool general = true;
   if (low > -CUDART_INF_F && n <= K) {
     // Every score is selected.
     for (int i = begin + tid; i < end; i += T) o[i] = i;
@@ -490,98 +506,151 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
     // 2^23 plus the bin of a score, rounded: non-decreasing in the score.
     auto place = [&](float a) { return fmaf(a - low, scale, kShift); };
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
+    for (int i = 0; i < kPer; ++i) {
+      if (i > last) break;
       if (i < rounds)
         atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place(v[i]))], 1u);
+    }
     find_bin<T, C>(s, need);
     const float bin = kShift + (float)(kBins - 1 - (int)s.bin);
     need -= s.above;
     uint32_t inside = s.inside;
-    // A second histogram over the bin's scores: bin - 0.5 .. bin + 0.5 of the
-    // first, cut to its 1024 bins, is non-decreasing in the score again.
+    // A histogram inside of the bin: bin - 0.5 .. bin + 0.5 of the first, cut
+    // to 1024 bins, is non-decreasing in the score again.
     const float edge = bin - kShift - 0.5f;
     auto place2 = [&](float a) {
       const float u = fmaf(a - low, scale, -edge);
       return fminf(fmaxf(u * (float)kBins, 0.0f), (float)(kBins - 1)) + kShift;
     };
-    float bin2 = 0.0f;
-    const bool twice = inside > need && inside > kList;
+    float bin2 = kShift;
+    const bool twice = inside > need && inside > kCand;
     if (twice) {
       row_sync<C>();  // every block has read the first histogram
       for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
+      for (int i = 0; i < kPer; ++i) {
+        if (i > last) break;
         if (i < rounds && place(v[i]) == bin)
           atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place2(v[i]))], 1u);
+      }
       find_bin<T, C>(s, need);
       bin2 = kShift + (float)(kBins - 1 - (int)s.bin);
       need -= s.above;
       inside = s.inside;
     }
-    if (inside <= kList) {
+    if (inside == need || inside <= kCand) {
+      const bool all = inside == need;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        if (i < rounds && place(v[i]) == bin && (!twice || place2(v[i]) == bin2)) {
-          const uint32_t p = (uint32_t)(begin + i * T + tid);
-          // -0 as +0, so that words of equal scores are equal.
-          const uint32_t a = __float_as_uint(v[i] + 0.0f);
-          if constexpr (C == 1) {
-            const uint32_t l = atomicAdd(&s.listed, 1u);
-            s.key[l] = a;
-            s.pos[l] = p;
-          } else {
-            const uint32_t l = peer_add(&s.listed, 0, 1u);
-            peer_store(&s.list_key[l], 0, a);
-            peer_store(&s.list_pos[l], 0, p);
+        if (i > last) break;
+        const float t = place(v[i]);
+        if (i < rounds && t >= bin) {
+          float d = t - bin;  // of the border: above or inside of bin2
+          if (twice && d == 0.0f) d = place2(v[i]) - bin2;
+          if (d > 0.0f || (all && d == 0.0f)) {
+            sel |= 1u << i;
+          } else if (d == 0.0f) {
+            // -0 as +0, so that words of equal scores are equal.
+            const uint32_t a = __float_as_uint(v[i] + 0.0f), p = (uint32_t)(begin + i * T + tid);
+            if constexpr (C == 1) {
+              const uint32_t l = atomicAdd(&s.listed, 1u);
+              s.list_key[l] = a;
+              s.list_pos[l] = p;
+            } else {
+              const uint32_t l = peer_add(&s.listed, 0, 1u);
+              peer_store(&s.list_key[l], 0, a);
+              peer_store(&s.list_pos[l], 0, p);
+            }
           }
         }
       }
-      row_sync<C>();
-      if constexpr (C > 1) {
-        if (tid < (int)inside) {
-          s.key[tid] = peer_load(&s.list_key[tid], 0);
-          s.pos[tid] = peer_load(&s.list_pos[tid], 0);
+      general = false;
+      if (!all) {
+        row_sync<C>();
+        const uint32_t* keys = s.list_key;
+        const uint32_t* poss = s.list_pos;
+        if constexpr (C > 1) {
+          for (int i = tid; i < (int)inside; i += T) {
+            s.mine_key[i] = peer_load(&s.list_key[i], 0);
+            s.mine_pos[i] = peer_load(&s.list_pos[i], 0);
+          }
+          keys = s.mine_key;
+          poss = s.mine_pos;
         }
-        __syncthreads();
+        // What the list's entries are told apart by: their bin inside of the
+        // border bin (or of bin2), then (score, position).
+        const float edge3 = twice ? bin2 - kShift - 0.5f : 0.0f;
+        auto place3 = [&](float a) {
+          const float u = fmaf(a - low, scale, -edge) * (float)kBins;
+          const float w = twice ? (u - edge3) * (float)kBins : u;
+          return fminf(fmaxf(w, 0.0f), (float)(kBins - 1)) + kShift;
+        };
+        float bin3 = 0.0f;  // every entry's bin is above it
+        uint32_t left = inside;
+        const bool thrice = inside > 32;
+        if (thrice) {
+          for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+          __syncthreads();
+          for (int i = tid; i < (int)inside; i += T)
+            atomicAdd(&s.hist[kShiftBits + (kBins - 1) -
+                              __float_as_uint(place3(__uint_as_float(keys[i])))],
+                      1u);
+          find_bin<T, C, true>(s, need);
+          bin3 = kShift + (float)(kBins - 1 - (int)s.bin);
+          need -= s.above;
+          left = s.inside;
+        } else if constexpr (C > 1) {
+          __syncthreads();
+        }
+        if (left > kList) {
+          general = true;  // the same in every block of the row
+        } else {
+          auto take = [&](uint32_t p) {
+            const uint32_t q = p - (uint32_t)begin;
+            if (p >= (uint32_t)begin && p < (uint32_t)end)
+              atomicOr(&s.taken[q % T], 1u << (q / T));
+          };
+          for (int i = tid; i < (int)inside; i += T) {
+            const float d = thrice ? place3(__uint_as_float(keys[i])) - bin3 : 0.0f;
+            if (d > 0.0f) {
+              take(poss[i]);
+            } else if (d == 0.0f) {
+              const uint32_t l = atomicAdd(&s.ranked, 1u);
+              s.key[l] = keys[i];
+              s.pos[l] = poss[i];
+            }
+          }
+          __syncthreads();
+          if (tid < (int)left) {
+            const float a = __uint_as_float(s.key[tid]);
+            const uint32_t p = s.pos[tid];
+            uint32_t r = 0;
+            for (int j = 0; j < (int)left; ++j) {
+              const float b = __uint_as_float(s.key[j]);
+              r += b > a || (b == a && s.pos[j] < p) ? 1u : 0u;
+            }
+            if (r < need) take(p);
+          }
+          __syncthreads();
+          sel |= s.taken[tid];
+        }
       }
-      if (tid < (int)inside) {
-        const float a = __uint_as_float(s.key[tid]);
-        const uint32_t p = s.pos[tid];
-        uint32_t r = 0;
-        for (int j = 0; j < (int)inside; ++j) {
-          const float b = __uint_as_float(s.key[j]);
-          r += b > a || (b == a && s.pos[j] < p) ? 1u : 0u;
-        }
-        if (r + 1 == need) {
-          s.thr_key = s.key[tid];
-          s.thr_pos = p;
-        }
-      }
-      __syncthreads();
-      const float threshold = __uint_as_float(s.thr_key);
-      // Rounds in which an equal score is still taken.
-      const int last = (int)s.thr_pos - begin - tid;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i < rounds && (v[i] > threshold || (v[i] == threshold && i * T <= last)))
-          sel |= 1u << i;
-    } else {
-      general = true;
     }
-  } else {
-    general = true;
   }
   if (general) {
     row_sync<C>();
+    if (tid == 0) s.listed = 0;
     sel = select_general<T, C>(s, x, begin, end, rank, K, &able);
   }
 
   uint32_t at[kPer], base;
-  count_before<T, C>(s, rank, sel, at, &base);
+  count_before<T, C>(s, rank, sel, last, at, &base);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
+  for (int i = 0; i < kPer; ++i) {
+    if (i > last) break;
     if (sel >> i & 1) o[base + at[i]] = begin + i * T + tid;
+  }
   const uint32_t filled = min(able, (uint32_t)K);
   for (uint32_t i = filled + rank * T + tid; i < (uint32_t)K; i += C * T) o[i] = -1;
   if constexpr (C > 1) row_sync<C>();  // no block leaves while another reads its shared memory
