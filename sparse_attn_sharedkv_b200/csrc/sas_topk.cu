@@ -27,10 +27,11 @@
 // until 128 or a single key are left; equal keys are taken by a count over
 // their positions.
 //
-// Thread t of a block holds the positions at a stride of T: loads are
-// coalesced for any row alignment.  The flags of four rounds are four bytes of
-// a word, so one shuffle scan counts them, and the selected lanes of a round
-// write neighbouring words.
+// Each warp of a block holds neighbouring positions, 32 a round: loads are
+// coalesced for any row alignment, the count of the selected positions before
+// a warp's is one number, and the selected lanes of a round write neighbouring
+// words.  The flags of four rounds are four bytes of a word, so one shuffle
+// scan counts them.
 
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -96,7 +97,6 @@ __device__ __forceinline__ void row_sync() {
 template <int T, int C>
 struct TopkShared {
   alignas(16) uint32_t hist[kBins];  // from the top bin down
-  alignas(16) uint32_t wtot[kPer * (T / 32)];
   uint32_t wmin[T / 32], wmax[T / 32], wcnt[T / 32], wsum[T / 32];
   uint32_t rmin[C], rmax[C], rcnt[C], rtot[C];  // one entry per block of the cluster
   uint32_t bin, above, inside;                  // found in the histogram, bin from the top
@@ -106,6 +106,24 @@ struct TopkShared {
   uint32_t key[kList], pos[kList];
   uint32_t taken[T];  // listed scores of each thread that are selected
   uint32_t thr_key, thr_pos;
+};
+
+// Positions of a block: `len` from `begin` on, `seg` for each warp.
+struct Places {
+  int begin, len, seg, last;  // the warps' rounds are 0 .. last
+
+  __device__ __forceinline__ Places(int begin_, int end, int threads)
+      : begin(begin_), len(end - begin_), last(max(0, (end - begin_ - 1) / threads)) {
+    seg = (last + 1) * 32;
+  }
+  // Rounds in which the thread holds a position, and the position.
+  __device__ __forceinline__ int rounds() const {
+    const int rest = len - (int)(threadIdx.x >> 5) * seg - (int)(threadIdx.x & 31);
+    return max(0, min(last + 1, (rest + 31) >> 5));
+  }
+  __device__ __forceinline__ int at(int i) const {
+    return begin + (int)(threadIdx.x >> 5) * seg + i * 32 + (int)(threadIdx.x & 31);
+  }
 };
 
 // Least and greatest of the keys (kmin, kmax) and the sum of n over the row's
@@ -186,16 +204,15 @@ __device__ __forceinline__ void find_bin(TopkShared<T, C>& s, uint32_t need) {
   __syncthreads();
 }
 
-// Count, over the row's positions, of the flags (bit i: the thread's key of
-// round i, none behind round `last`) before each of the thread's keys: at[i] for round i.  Returns the
-// block's total and, in *block_base, the count in the blocks before it.
+// Count, over the row's positions, of the flags (bit i: the thread's position
+// of round i, none behind round `last`) before each of the thread's positions:
+// at[i] for round i, the blocks before this one included.
 template <int T, int C>
-__device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, uint32_t flags,
-                                                 int last, uint32_t (&at)[kPer],
-                                                 uint32_t* block_base) {
-  constexpr int W = T / 32, kChunk = W / 2;  // kPer * W counts: kChunk of them a lane
+__device__ __forceinline__ void count_before(TopkShared<T, C>& s, int rank, uint32_t flags,
+                                             int last, uint32_t (&at)[kPer]) {
+  constexpr int W = T / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t incl4[kPer / 4] = {};
+  uint32_t sum = 0;  // of the warp's rounds so far
 #pragma unroll
   for (int g = 0; g < kPer / 4; ++g) {
     if (4 * g > last) break;
@@ -207,58 +224,42 @@ __device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, 
       const uint32_t up = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += up;
     }
-    incl4[g] = v;
+    const uint32_t total = __shfl_sync(0xffffffffu, v, 31);
+    v -= own;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) at[4 * g + k] = ((v - own) >> (8 * k)) & 255u;
+    for (int k = 0; k < 4; ++k) {
+      at[4 * g + k] = sum + ((v >> (8 * k)) & 255u);
+      sum += (total >> (8 * k)) & 255u;
+    }
   }
   __syncthreads();
-  if (lane == 31) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) s.wtot[i * W + warp] = (incl4[i / 4] >> (8 * (i % 4))) & 255u;
-  }
+  if (lane == 0) s.wsum[warp] = sum;
   __syncthreads();
-  // Lane l: counts l kChunk .. of the rounds in order, their sum and the part
-  // before this warp's inside the chunk.
-  uint32_t sum = 0, part = 0;
-#pragma unroll
-  for (int k = 0; k < kChunk; ++k) {
-    const uint32_t v = s.wtot[lane * kChunk + k];
-    part += k < warp % kChunk ? v : 0u;
-    sum += v;
+  const uint32_t other = lane < W ? s.wsum[lane] : 0u;
+  uint32_t base = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0u);
+  if constexpr (C > 1) {
+    const uint32_t total = __reduce_add_sync(0xffffffffu, other);
+    if (warp == 0 && lane < C) peer_store(&s.rtot[rank], lane, total);
+    row_sync<C>();
+    base += __reduce_add_sync(0xffffffffu, lane < rank ? s.rtot[lane] : 0u);
   }
-  uint32_t incl = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  const uint32_t start = incl - sum + part;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (i > last) break;
-    at[i] += __shfl_sync(0xffffffffu, start, 2 * i + (warp >= kChunk ? 1 : 0));
+    at[i] += base;
   }
-  const uint32_t total = __shfl_sync(0xffffffffu, incl, 31);
-  *block_base = 0;
-  if constexpr (C > 1) {
-    if (warp == 0 && lane < C) peer_store(&s.rtot[rank], lane, total);
-    row_sync<C>();
-    *block_base = __reduce_add_sync(0xffffffffu, lane < rank ? s.rtot[lane] : 0u);
-  }
-  return total;
 }
 
 // Selection flags of any row, by keys.  Shared memory is in use up to here by
 // no thread of the row.
 template <int T, int C>
-__device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float* x, int begin,
-                                                int end, int rank, int K, uint32_t* selectable) {
-  const int tid = threadIdx.x;
+__device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float* x, Places pl,
+                                                int rank, int K, uint32_t* selectable) {
+  const int tid = threadIdx.x, rounds = pl.rounds();
   uint32_t key[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int p = begin + i * T + tid;
-    key[i] = p < end ? key_of(__ldg(x + p)) : 0u;
+    key[i] = i < rounds ? key_of(__ldg(x + pl.at(i))) : 0u;
   }
   for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
 
@@ -349,17 +350,17 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       sel |= cand;
     } else if (equal) {
       // The first `need` of the equal keys by position.
-      uint32_t at[kPer], base;
-      count_before<T, C>(s, rank, cand, kPer - 1, at, &base);
+      uint32_t at[kPer];
+      count_before<T, C>(s, rank, cand, kPer - 1, at);
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (cand >> i & 1) sel |= (base + at[i] < need ? 1u : 0u) << i;
+        if (cand >> i & 1) sel |= (at[i] < need ? 1u : 0u) << i;
       row_sync<C>();  // before the counts are written again
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         if (cand >> i & 1) {
-          const uint32_t p = (uint32_t)(begin + i * T + tid);
+          const uint32_t p = (uint32_t)pl.at(i);
           if constexpr (C == 1) {
             const uint32_t l = atomicAdd(&s.listed, 1u);
             s.key[l] = key[i];
@@ -394,7 +395,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         if (cand >> i & 1) {
-          const uint32_t p = (uint32_t)(begin + i * T + tid);
+          const uint32_t p = (uint32_t)pl.at(i);
           sel |= (key[i] > tk || (key[i] == tk && p <= tp) ? 1u : 0u) << i;
         }
       }
@@ -449,11 +450,10 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
     for (int i = rank * T + tid; i < K; i += C * T) o[i] = -1;
     return;
   }
-  // The block's part of the row; the thread holds a score in `rounds` rounds,
-  // some thread does up to round `last`.
-  const int part = (n + C - 1) / C;
+  const int part = (n + C - 1) / C;  // of the block
   const int begin = min(n, rank * part), end = min(n, begin + part);
-  const int rounds = (end - begin - tid + T - 1) / T, last = (end - begin - 1) / T;
+  const Places pl(begin, end, T);
+  const int rounds = pl.rounds(), last = pl.last;
 
   // Empty places hold the row's first score, which changes no extremum.
   const float first = __ldg(x);
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (i > last) break;
-    v[i] = i < rounds ? __ldg(x + begin + i * T + tid) : first;
+    v[i] = i < rounds ? __ldg(x + pl.at(i)) : first;
   }
   for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
   s.taken[tid] = 0;
@@ -541,29 +541,56 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
     }
     if (inside == need || inside <= kCand) {
       const bool all = inside == need;
+      uint32_t cand = 0;  // of the border
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         if (i > last) break;
         const float t = place(v[i]);
-        if (i < rounds && t >= bin) {
-          float d = t - bin;  // of the border: above or inside of bin2
-          if (twice && d == 0.0f) d = place2(v[i]) - bin2;
-          if (d > 0.0f || (all && d == 0.0f)) {
-            sel |= 1u << i;
-          } else if (d == 0.0f) {
-            // -0 as +0, so that words of equal scores are equal.
-            const uint32_t a = __float_as_uint(v[i] + 0.0f), p = (uint32_t)(begin + i * T + tid);
-            if constexpr (C == 1) {
-              const uint32_t l = atomicAdd(&s.listed, 1u);
-              s.list_key[l] = a;
-              s.list_pos[l] = p;
-            } else {
-              const uint32_t l = peer_add(&s.listed, 0, 1u);
-              peer_store(&s.list_key[l], 0, a);
-              peer_store(&s.list_pos[l], 0, p);
-            }
+        sel |= (t > bin ? 1u : 0u) << i;
+        cand |= (t == bin ? 1u : 0u) << i;
+      }
+      const uint32_t valid = (1u << rounds) - 1u;
+      sel &= valid;
+      cand &= valid;
+      if (twice || !all) {
+        // Few of the border a thread: looked at one by one, read again.
+        const int count = __popc(cand);
+        uint32_t slot = 0;
+        if (!twice) {
+          // A place for each in the list.
+          uint32_t incl = (uint32_t)count;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += up;
           }
+          if (lane == 31 && incl > 0)
+            slot = C == 1 ? atomicAdd(&s.listed, incl) : peer_add(&s.listed, 0, incl);
+          slot = __shfl_sync(0xffffffffu, slot, 31) + incl - (uint32_t)count;
         }
+        for (uint32_t rest = cand; rest != 0; rest &= rest - 1) {
+          const int i = __ffs(rest) - 1;
+          const uint32_t p = (uint32_t)pl.at(i);
+          const float a = __ldg(x + p);
+          if (twice) {
+            const float d = place2(a) - bin2;
+            if (d > 0.0f || (all && d == 0.0f)) sel |= 1u << i;
+            if (d != 0.0f || all) continue;
+            slot = C == 1 ? atomicAdd(&s.listed, 1u) : peer_add(&s.listed, 0, 1u);
+          }
+          // -0 as +0, so that words of equal scores are equal.
+          const uint32_t word = __float_as_uint(a + 0.0f);
+          if constexpr (C == 1) {
+            s.list_key[slot] = word;
+            s.list_pos[slot] = p;
+          } else {
+            peer_store(&s.list_key[slot], 0, word);
+            peer_store(&s.list_pos[slot], 0, p);
+          }
+          ++slot;
+        }
+      } else {
+        sel |= cand;
       }
       general = false;
       if (!all) {
@@ -607,9 +634,9 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
           general = true;  // the same in every block of the row
         } else {
           auto take = [&](uint32_t p) {
-            const uint32_t q = p - (uint32_t)begin;
-            if (p >= (uint32_t)begin && p < (uint32_t)end)
-              atomicOr(&s.taken[q % T], 1u << (q / T));
+            if ((int)p < begin || (int)p >= end) return;
+            const int q = (int)p - begin, w = q / pl.seg, r = q - w * pl.seg;
+            atomicOr(&s.taken[w * 32 + (r & 31)], 1u << (r >> 5));
           };
           for (int i = tid; i < (int)inside; i += T) {
             const float d = thrice ? place3(__uint_as_float(keys[i])) - bin3 : 0.0f;
@@ -641,15 +668,15 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
   if (general) {
     row_sync<C>();
     if (tid == 0) s.listed = 0;
-    sel = select_general<T, C>(s, x, begin, end, rank, K, &able);
+    sel = select_general<T, C>(s, x, pl, rank, K, &able);
   }
 
-  uint32_t at[kPer], base;
-  count_before<T, C>(s, rank, sel, last, at, &base);
+  uint32_t at[kPer];
+  count_before<T, C>(s, rank, sel, last, at);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (i > last) break;
-    if (sel >> i & 1) o[base + at[i]] = begin + i * T + tid;
+    if (sel >> i & 1) o[at[i]] = pl.at(i);
   }
   const uint32_t filled = min(able, (uint32_t)K);
   for (uint32_t i = filled + rank * T + tid; i < (uint32_t)K; i += C * T) o[i] = -1;
