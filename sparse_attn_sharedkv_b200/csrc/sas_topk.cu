@@ -428,10 +428,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// 1280 threads an SM where the block size allows: 48 registers a thread, which
-// hold the ordinary path without spills.
+// One block a row: as many blocks as the SM has threads for (32 registers, a
+// few of them spilled), since a row is a chain of short phases: 32768 rows of up
+// to 4096 take 214 us so, 251 us at 1280 threads an SM without spills.
 template <int T, int C>
-__global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C, 1, 1)
+__global__ void __launch_bounds__(T, C == 1 ? 2048 / T : 1) __cluster_dims__(C, 1, 1)
     topk_kernel(const float* __restrict__ scores, int64_t stride,
                 const int32_t* __restrict__ lengths, int n_cols, int K,
                 int32_t* __restrict__ out) {
@@ -464,15 +465,24 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
     if (i > last) break;
     v[i] = i < rounds ? __ldg(x + pl.at(i)) : first;
   }
-  for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
-  s.taken[tid] = 0;
-  if (tid == 0) s.listed = s.ranked = 0;
+  const bool short_row = n <= K;
+  if (short_row) {
+    // Every score is selected, unless one of them turns out to be -inf: the
+    // positions are on their way before the scores are here.
+    for (int i = begin + tid; i < end; i += T) o[i] = i;
+    for (int i = n + rank * T + tid; i < K; i += C * T) o[i] = -1;
+  } else {
+    for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+    s.taken[tid] = 0;
+    if (tid == 0) s.listed = s.ranked = 0;
+  }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (i > last) break;
     low = min_nan(low, v[i]);
     high = max_nan(high, v[i]);
   }
+  if (C == 1 && short_row && !__syncthreads_or(!(low > -CUDART_INF_F))) return;
   low = warp_min(low);
   high = warp_max(high);
   if (lane == 0) {
@@ -495,13 +505,9 @@ __global__ void __launch_bounds__(T, T <= 512 ? 1280 / T : 1) __cluster_dims__(C
   uint32_t sel = 0, able = (uint32_t)n;  // bit i of sel: v[i] is selected
   const float scale = __fdividef((float)(kBins - 2), high - low);
   bool general = true;
-  if (low > -CUDART_INF_F && n <= K) {
-    // Every score is selected.
-    for (int i = begin + tid; i < end; i += T) o[i] = i;
-    for (int i = n + rank * T + tid; i < K; i += C * T) o[i] = -1;
-    return;
-  }
-  if (low > -CUDART_INF_F && high < CUDART_INF_F && scale > 0.0f && scale < CUDART_INF_F) {
+  if (short_row && low > -CUDART_INF_F) return;
+  if (!short_row && low > -CUDART_INF_F && high < CUDART_INF_F && scale > 0.0f &&
+      scale < CUDART_INF_F) {
     uint32_t need = (uint32_t)K;
     // 2^23 plus the bin of a score, rounded: non-decreasing in the score.
     auto place = [&](float a) { return fmaf(a - low, scale, kShift); };
