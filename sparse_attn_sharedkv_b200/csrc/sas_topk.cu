@@ -38,13 +38,13 @@
 #include <stdint.h>
 
 #include "sas.h"
+#include "sas_kernels.h"
 
 namespace {
 
 constexpr int kBins = 1024;
 constexpr int kCand = 512;                 // border scores listed
 constexpr int kList = 128;                 // keys ranked directly
-constexpr int kPer = 16;                   // keys of a thread
 constexpr uint32_t kNegInf = 0x007fffffu;  // key of -inf
 constexpr uint32_t kPosInf = 0xff800000u;  // key of +inf
 
@@ -207,14 +207,14 @@ __device__ __forceinline__ void find_bin(TopkShared<T, C>& s, uint32_t need) {
 // Count, over the row's positions, of the flags (bit i: the thread's position
 // of round i, none behind round `last`) before each of the thread's positions:
 // at[i] for round i, the blocks before this one included.
-template <int T, int C>
+template <int T, int C, int P>
 __device__ __forceinline__ void count_before(TopkShared<T, C>& s, int rank, uint32_t flags,
-                                             int last, uint32_t (&at)[kPer]) {
+                                             int last, uint32_t (&at)[P]) {
   constexpr int W = T / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t sum = 0;  // of the warp's rounds so far
 #pragma unroll
-  for (int g = 0; g < kPer / 4; ++g) {
+  for (int g = 0; g < P / 4; ++g) {
     if (4 * g > last) break;
     // Bits 0 .. 3 of the group into the low bits of four bytes.
     const uint32_t own = ((flags >> (4 * g) & 15u) * 0x00204081u) & 0x01010101u;
@@ -244,7 +244,7 @@ __device__ __forceinline__ void count_before(TopkShared<T, C>& s, int rank, uint
     base += __reduce_add_sync(0xffffffffu, lane < rank ? s.rtot[lane] : 0u);
   }
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < P; ++i) {
     if (i > last) break;
     at[i] += base;
   }
@@ -252,20 +252,20 @@ __device__ __forceinline__ void count_before(TopkShared<T, C>& s, int rank, uint
 
 // Selection flags of any row, by keys.  Shared memory is in use up to here by
 // no thread of the row.
-template <int T, int C>
+template <int T, int C, int P>
 __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float* x, Places pl,
                                                 int rank, int K, uint32_t* selectable) {
   const int tid = threadIdx.x, rounds = pl.rounds();
-  uint32_t key[kPer];
+  uint32_t key[P];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < P; ++i) {
     key[i] = i < rounds ? key_of(__ldg(x + pl.at(i))) : 0u;
   }
   for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
 
   uint32_t kmin = 0xffffffffu, kmax = 0, able = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < P; ++i) {
     if (key[i] > kNegInf) {
       ++able;
       if (key[i] < kPosInf) {
@@ -279,7 +279,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
   uint32_t sel = 0;  // bit i: key[i] is selected
   if (able <= (uint32_t)K) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sel |= (key[i] > kNegInf ? 1u : 0u) << i;
+    for (int i = 0; i < P; ++i) sel |= (key[i] > kNegInf ? 1u : 0u) << i;
   } else {
     // Linear in the scores; a range whose scale is not finite (it overflows,
     // is subnormal or a single value) puts every finite score into the last bin.
@@ -292,7 +292,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       return kBins - 1 - (int)fminf(fmaxf((score_of(k) - low) * scale, 0.0f), (float)(kBins - 1));
     };
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
+    for (int i = 0; i < P; ++i)
       if (key[i] > kNegInf) atomicAdd(&s.hist[bin_of(key[i])], 1u);
     uint32_t need = (uint32_t)K;
     find_bin<T, C>(s, need);
@@ -301,7 +301,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
     need -= s.above;
     uint32_t inside = s.inside;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < P; ++i) {
       if (key[i] > kNegInf) {
         const int b = bin_of(key[i]);
         sel |= (b < bin ? 1u : 0u) << i;
@@ -314,7 +314,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       kmax = 0;
       uint32_t none = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < P; ++i) {
         if (cand >> i & 1) {
           kmin = min(kmin, key[i]);
           kmax = max(kmax, key[i]);
@@ -331,14 +331,14 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       __syncthreads();
       const int shift = max(0, 22 - __clz(kmax - kmin));  // range >> shift below 1024
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
+      for (int i = 0; i < P; ++i)
         if (cand >> i & 1) atomicAdd(&s.hist[kBins - 1 - (int)((key[i] - kmin) >> shift)], 1u);
       find_bin<T, C>(s, need);
       bin = (int)s.bin;
       need -= s.above;
       inside = s.inside;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < P; ++i) {
         if (cand >> i & 1) {
           const int b = kBins - 1 - (int)((key[i] - kmin) >> shift);
           sel |= (b < bin ? 1u : 0u) << i;
@@ -350,15 +350,15 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       sel |= cand;
     } else if (equal) {
       // The first `need` of the equal keys by position.
-      uint32_t at[kPer];
-      count_before<T, C>(s, rank, cand, kPer - 1, at);
+      uint32_t at[P];
+      count_before<T, C>(s, rank, cand, P - 1, at);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
+      for (int i = 0; i < P; ++i)
         if (cand >> i & 1) sel |= (at[i] < need ? 1u : 0u) << i;
       row_sync<C>();  // before the counts are written again
     } else {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < P; ++i) {
         if (cand >> i & 1) {
           const uint32_t p = (uint32_t)pl.at(i);
           if constexpr (C == 1) {
@@ -393,7 +393,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       __syncthreads();
       const uint32_t tk = s.thr_key, tp = s.thr_pos;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < P; ++i) {
         if (cand >> i & 1) {
           const uint32_t p = (uint32_t)pl.at(i);
           sel |= (key[i] > tk || (key[i] == tk && p <= tp) ? 1u : 0u) << i;
@@ -431,8 +431,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // One block a row: as many blocks as the SM has threads for (32 registers, a
 // few of them spilled), since a row is a chain of short phases: 32768 rows of up
 // to 4096 take 214 us so, 251 us at 1280 threads an SM without spills.
-template <int T, int C>
-__global__ void __launch_bounds__(T, C == 1 ? 2048 / T : 1) __cluster_dims__(C, 1, 1)
+template <int T, int C, int P>
+__global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster_dims__(C, 1, 1)
     topk_kernel(const float* __restrict__ scores, int64_t stride,
                 const int32_t* __restrict__ lengths, int n_cols, int K,
                 int32_t* __restrict__ out) {
@@ -458,10 +458,10 @@ __global__ void __launch_bounds__(T, C == 1 ? 2048 / T : 1) __cluster_dims__(C, 
 
   // Empty places hold the row's first score, which changes no extremum.
   const float first = __ldg(x);
-  float v[kPer];
+  float v[P];
   float low = first, high = first;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < P; ++i) {
     if (i > last) break;
     v[i] = i < rounds ? __ldg(x + pl.at(i)) : first;
   }
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(T, C == 1 ? 2048 / T : 1) __cluster_dims__(C, 
     if (tid == 0) s.listed = s.ranked = 0;
   }
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < P; ++i) {
     if (i > last) break;
     low = min_nan(low, v[i]);
     high = max_nan(high, v[i]);
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(T, C == 1 ? 2048 / T : 1) __cluster_dims__(C, 
     // 2^23 plus the bin of a score, rounded: non-decreasing in the score.
     auto place = [&](float a) { return fmaf(a - low, scale, kShift); };
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < P; ++i) {
       if (i > last) break;
       if (i < rounds)
         atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place(v[i]))], 1u);
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(T, C == 1 ? 2048 / T : 1) __cluster_dims__(C, 
       for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < P; ++i) {
         if (i > last) break;
         if (i < rounds && place(v[i]) == bin)
           atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place2(v[i]))], 1u);
@@ -549,13 +549,13 @@ __global__ void __launch_bounds__(T, C == 1 ? 2048 / T : 1) __cluster_dims__(C, 
       const bool all = inside == need;
       uint32_t cand = 0;  // of the border
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
+      for (int i = 0; i < P; ++i) {
         if (i > last) break;
         const float t = place(v[i]);
         sel |= (t > bin ? 1u : 0u) << i;
         cand |= (t == bin ? 1u : 0u) << i;
       }
-      const uint32_t valid = (1u << rounds) - 1u;
+      const uint32_t valid = rounds < 32 ? (1u << rounds) - 1u : 0xffffffffu;
       sel &= valid;
       cand &= valid;
       if (twice || !all) {
@@ -674,13 +674,13 @@ __global__ void __launch_bounds__(T, C == 1 ? 2048 / T : 1) __cluster_dims__(C, 
   if (general) {
     row_sync<C>();
     if (tid == 0) s.listed = 0;
-    sel = select_general<T, C>(s, x, pl, rank, K, &able);
+    sel = select_general<T, C, P>(s, x, pl, rank, K, &able);
   }
 
-  uint32_t at[kPer];
+  uint32_t at[P];
   count_before<T, C>(s, rank, sel, last, at);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int i = 0; i < P; ++i) {
     if (i > last) break;
     if (sel >> i & 1) o[at[i]] = pl.at(i);
   }
@@ -778,18 +778,26 @@ extern "C" int sas_topk_select(const float* scores, int64_t score_stride, const 
   if (!indices || (num_keys > 0 && !scores)) return SAS_ERR_INVALID;
   if (rows > INT32_MAX / 8) return SAS_ERR_UNSUPPORTED;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  // The smallest block whose registers hold the row, then clusters of blocks
-  // of 512 threads (8192 keys), then of 1024.
-#define SAS_TOPK(T, C)                                                                           \
-  topk_kernel<T, C><<<(unsigned)rows * C, T, 0, stream>>>(scores, score_stride, lengths, num_keys, \
-                                                          topk, indices)
-  if (num_keys <= kPer * 128) SAS_TOPK(128, 1);
-  else if (num_keys <= kPer * 256) SAS_TOPK(256, 1);
-  else if (num_keys <= kPer * 512) SAS_TOPK(512, 1);
-  else if (num_keys <= kPer * 512 * 2) SAS_TOPK(512, 2);
-  else if (num_keys <= kPer * 512 * 4) SAS_TOPK(512, 4);
-  else if (num_keys <= kPer * 512 * 8) SAS_TOPK(512, 8);
-  else if (num_keys <= kPer * 1024 * 8) SAS_TOPK(1024, 8);
+  // The smallest block whose registers hold the row, or a cluster of as few of
+  // the largest as it takes (a cluster's barriers and remote reads cost more
+  // than a block's longer phases: 256 rows of 32768 take 29 us in blocks of 1024
+  // threads and 86 us in clusters of four of 512) unless the rows are so few
+  // that the clusters fit the SMs side by side.
+#define SAS_TOPK(T, C, P)                                                                          \
+  topk_kernel<T, C, P><<<(unsigned)rows * C, T, 0, stream>>>(scores, score_stride, lengths,        \
+                                                             num_keys, topk, indices)
+  int dev = 0;
+  const int sms = sas::current_device_sms(&dev);
+  if (sms <= 0) return SAS_ERR_CUDA;
+  const bool few = (int64_t)rows * 4 <= sms;
+  if (num_keys <= 16 * 128) SAS_TOPK(128, 1, 16);
+  else if (num_keys <= 16 * 256) SAS_TOPK(256, 1, 16);
+  else if (num_keys <= 16 * 512) SAS_TOPK(512, 1, 16);
+  else if (num_keys <= 16 * 1024) SAS_TOPK(1024, 1, 16);
+  else if (num_keys <= 32 * 1024 && few) SAS_TOPK(512, 4, 16);
+  else if (num_keys <= 32 * 1024) SAS_TOPK(1024, 1, 32);
+  else if (num_keys <= 32 * 1024 * 2) SAS_TOPK(1024, 2, 32);
+  else if (num_keys <= 32 * 1024 * 4) SAS_TOPK(1024, 4, 32);
   else
     topk_long_kernel<<<rows, kLongThreads, 0, stream>>>(scores, score_stride, lengths, num_keys,
                                                         topk, indices);

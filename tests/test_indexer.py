@@ -372,7 +372,8 @@ KINDS = ("normal", "ties", "equal", "two", "wide", "close", "tiny", "outlier", "
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("rows, N, K", [(1, 1, 1), (3, 5, 9), (2, 100, 100), (5, 513, 64),
                                         (3, 2049, 2048), (4, 4096, 1), (2, 4097, 512),
-                                        (3, 9000, 2048), (2, 33000, 2000), (1, 140001, 2048),
+                                        (3, 9000, 2048), (2, 17001, 700), (60, 16390, 100),
+                                        (2, 33000, 2000), (2, 131072, 2048), (1, 140001, 2048),
                                         (300, 700, 130)])
 def test_gpu_select_topk(rows, N, K, kind):
     g = torch.Generator().manual_seed(N + K)
