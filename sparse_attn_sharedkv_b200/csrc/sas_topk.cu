@@ -158,6 +158,12 @@ __device__ __forceinline__ void row_reduce(TopkShared<T, C>& s, int rank, uint32
   }
 }
 
+template <int T, int C>
+__device__ __forceinline__ void clear_histogram(TopkShared<T, C>& s) {
+  uint4* h = reinterpret_cast<uint4*>(s.hist);
+  for (int i = threadIdx.x; i < kBins / 4; i += T) h[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 // The bin of the histograms (of all the row's blocks) in which the need-th
 // largest lies: into s.bin, with the count above it and the one inside.
 // Starts and ends with a barrier of the row / the block.
@@ -206,10 +212,10 @@ __device__ __forceinline__ void find_bin(TopkShared<T, C>& s, uint32_t need) {
 
 // Count, over the row's positions, of the flags (bit i: the thread's position
 // of round i, none behind round `last`) before each of the thread's positions:
-// at[i] for round i, the blocks before this one included.
+// the returned count, of the warps and blocks before, and at[i] for round i.
 template <int T, int C, int P>
-__device__ __forceinline__ void count_before(TopkShared<T, C>& s, int rank, uint32_t flags,
-                                             int last, uint32_t (&at)[P]) {
+__device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, uint32_t flags,
+                                                 int last, uint32_t (&at)[P]) {
   constexpr int W = T / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t sum = 0;  // of the warp's rounds so far
@@ -224,13 +230,12 @@ __device__ __forceinline__ void count_before(TopkShared<T, C>& s, int rank, uint
       const uint32_t up = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += up;
     }
+    // Bytes of the rounds before in the group; all stay below 128.
     const uint32_t total = __shfl_sync(0xffffffffu, v, 31);
-    v -= own;
+    v += total * 0x01010100u - own;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      at[4 * g + k] = sum + ((v >> (8 * k)) & 255u);
-      sum += (total >> (8 * k)) & 255u;
-    }
+    for (int k = 0; k < 4; ++k) at[4 * g + k] = sum + ((v >> (8 * k)) & 255u);
+    sum += (total * 0x01010101u) >> 24;
   }
   __syncthreads();
   if (lane == 0) s.wsum[warp] = sum;
@@ -243,11 +248,7 @@ __device__ __forceinline__ void count_before(TopkShared<T, C>& s, int rank, uint
     row_sync<C>();
     base += __reduce_add_sync(0xffffffffu, lane < rank ? s.rtot[lane] : 0u);
   }
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    if (i > last) break;
-    at[i] += base;
-  }
+  return base;
 }
 
 // Selection flags of any row, by keys.  Shared memory is in use up to here by
@@ -261,7 +262,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
   for (int i = 0; i < P; ++i) {
     key[i] = i < rounds ? key_of(__ldg(x + pl.at(i))) : 0u;
   }
-  for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+  clear_histogram<T, C>(s);
 
   uint32_t kmin = 0xffffffffu, kmax = 0, able = 0;
 #pragma unroll
@@ -327,7 +328,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       }
       // Every block of the row has read the histograms: its last barrier was
       // behind them.
-      for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+      clear_histogram<T, C>(s);
       __syncthreads();
       const int shift = max(0, 22 - __clz(kmax - kmin));  // range >> shift below 1024
 #pragma unroll
@@ -351,10 +352,10 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
     } else if (equal) {
       // The first `need` of the equal keys by position.
       uint32_t at[P];
-      count_before<T, C>(s, rank, cand, P - 1, at);
+      const uint32_t base = count_before<T, C>(s, rank, cand, P - 1, at);
 #pragma unroll
       for (int i = 0; i < P; ++i)
-        if (cand >> i & 1) sel |= (at[i] < need ? 1u : 0u) << i;
+        if (cand >> i & 1) sel |= (base + at[i] < need ? 1u : 0u) << i;
       row_sync<C>();  // before the counts are written again
     } else {
 #pragma unroll
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
     for (int i = begin + tid; i < end; i += T) o[i] = i;
     for (int i = n + rank * T + tid; i < K; i += C * T) o[i] = -1;
   } else {
-    for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+    clear_histogram<T, C>(s);
     s.taken[tid] = 0;
     if (tid == 0) s.listed = s.ranked = 0;
   }
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
     const bool twice = inside > need && inside > kCand;
     if (twice) {
       row_sync<C>();  // every block has read the first histogram
-      for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+      clear_histogram<T, C>(s);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < P; ++i) {
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
         uint32_t left = inside;
         const bool thrice = inside > 32;
         if (thrice) {
-          for (int i = tid; i < kBins; i += T) s.hist[i] = 0;
+          clear_histogram<T, C>(s);
           __syncthreads();
           for (int i = tid; i < (int)inside; i += T)
             atomicAdd(&s.hist[kShiftBits + (kBins - 1) -
@@ -678,11 +679,11 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
   }
 
   uint32_t at[P];
-  count_before<T, C>(s, rank, sel, last, at);
+  int32_t* dst = o + count_before<T, C>(s, rank, sel, last, at);
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     if (i > last) break;
-    if (sel >> i & 1) o[at[i]] = pl.at(i);
+    if (sel >> i & 1) dst[at[i]] = pl.at(i);
   }
   const uint32_t filled = min(able, (uint32_t)K);
   for (uint32_t i = filled + rank * T + tid; i < (uint32_t)K; i += C * T) o[i] = -1;
