@@ -237,6 +237,59 @@ def test_gpu_index_scores_special_values():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H", [12, 16, 20, 33, 64, 100, 128])
+def test_gpu_index_scores_infinite_key(H):
+    # An infinity in a seen key is that score's, also where the heads do not fill a tile.
+    g = torch.Generator().manual_seed(H)
+    q = torch.rand(1, H, 64, generator=g).to(torch.bfloat16) + 0.5
+    w = torch.rand(1, H, generator=g) + 0.5
+    pool = torch.rand(4, 64, 1, 64, generator=g).to(torch.bfloat16)
+    pool[1, 3] = float("inf")
+    s = run_scores((q, w, pool, torch.tensor([[2, 1, 0]], dtype=torch.int32), [0, 1], [150], 1,
+                    150))
+    assert s[0, 67] == float("inf") and s[0, :67].isfinite().all() and s[0, 68:].isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H, D, bs", [(16, 128, 64), (64, 128, 64), (128, 64, 48), (40, 128, 20)])
+def test_gpu_index_scores_long_runs(H, D, bs):
+    # Rows of 131072 keys, so that each pair of CTAs goes through its buffers many times, and
+    # groups of few and of many tokens in turn.
+    g = torch.Generator().manual_seed(H + bs)
+    B, N, per = 41, 131072, 2 * max(1, 128 // H)
+    q_len = torch.randint(1, per + 1, (B,), generator=g).tolist()
+    q_len[3:7] = [0, 1, 2 * per + 1, per]
+    kv = torch.randint(N // 2, N + 1, (B,), generator=g).tolist()
+    kv[5], kv[9], kv[11] = N, 77, 0
+    cu = [0] + torch.tensor(q_len).cumsum(0).tolist()
+    T, blocks, rows = cu[-1], 300, -(-N // bs)
+    q = torch.randn(T, H, D, generator=g).to(torch.bfloat16).cuda()
+    w = torch.randn(T, H, generator=g).cuda()
+    pool = torch.randn(blocks, bs, 1, D, generator=g).to(torch.bfloat16).cuda()
+    table = torch.randint(0, blocks, (B, rows), generator=g, dtype=torch.int32)
+    table[torch.rand(B, rows, generator=g) < 0.01] = -1
+    table = table.cuda()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()
+    got = indexer.index_scores(q, w, key_pool=pool, block_table=table, cu_seqlens_q=i32(cu),
+                               seqused_kv=i32(kv), max_keys=N)
+    j = torch.arange(N, device="cuda")
+    flat = pool.view(-1, D).double()
+    for b in range(B):
+        blk = table[b].long()[j // bs]
+        k = flat[blk.clamp(min=0) * bs + j % bs]
+        for s in range(q_len[b]):
+            t = cu[b] + s
+            none = (j >= kv[b] - q_len[b] + s + 1) | (blk < 0)
+            x = q[t].double()
+            want = w[t].double() @ torch.relu(x @ k.T)
+            mag = w[t].double().abs() @ (x.abs() @ k.abs().T)
+            assert torch.equal(got[t] == NEG, none), (b, s)
+            off = torch.where(none, 0.0, (got[t].double() - want).abs())
+            tol = (D + H + 2) * 2.0 ** -23 * mag + 1e-30  # as check_scores derives it
+            assert torch.all(off <= tol), (b, s, float((off / tol).max()))
+
+
+@pytest.mark.gpu
 def test_gpu_index_scores_bsnd_and_rows_of_no_sequence():
     case = score_case(11, (4, 4, 4), (300, 4, 150), 16, 64, 16)
     q, w, pool, table, cu, kv, _, N = case
