@@ -305,6 +305,7 @@ int sas_kv_append_norm_rope(const SasRowTransform* transform, void* pool, int32_
 
 #define SAS_MAX_INDEX_HEADS 128
 #define SAS_MAX_INDEX_DIM 128
+#define SAS_MAX_TOPK (1 << 30)
 
 /* Index scores of the tokens [first_token, first_token + num_tokens) against
  * the paged index keys of their sequences:

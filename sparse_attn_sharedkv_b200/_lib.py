@@ -29,6 +29,8 @@ SAS_MAX_ROW_DIM = 1024
 SAS_MAX_ROPE_DIM = 256
 SAS_MAX_INDEX_HEADS = 128
 SAS_MAX_INDEX_DIM = 128
+SAS_MAX_TOPK = 1 << 30
+INT32_MAX = 2 ** 31 - 1
 SAS_AIC_CORE_NUM = 36
 SAS_AIV_CORE_NUM = 72
 SAS_FA_METADATA_SIZE = 8

@@ -775,7 +775,8 @@ extern "C" int sas_index_scores(const SasIndexParams* params, void* stream_ptr) 
     return SAS_ERR_UNSUPPORTED;
   if (p.max_q_len > 0 && (int64_t)p.max_q_len * p.batch != p.total_tokens) return SAS_ERR_INVALID;
   if (p.num_tokens == 0 || (p.num_keys == 0 && !p.lengths)) return SAS_OK;
-  if (!p.q || !p.weights || !p.key_pool || !p.block_table || !p.kv_len || !p.scores ||
+  if (!p.q || !p.weights || !p.kv_len || (p.num_keys > 0 && !p.scores) ||
+      (p.num_blocks > 0 && !p.key_pool) || (p.table_len > 0 && !p.block_table) ||
       (p.max_q_len == 0 && !p.cu_seqlens_q))
     return SAS_ERR_INVALID;
   if (((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.key_pool)) & 15) != 0)

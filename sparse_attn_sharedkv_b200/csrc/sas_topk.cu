@@ -777,7 +777,9 @@ extern "C" int sas_topk_select(const float* scores, int64_t score_stride, const 
   if (rows < 0 || num_keys < 0 || topk < 1 || score_stride < num_keys) return SAS_ERR_INVALID;
   if (rows == 0) return SAS_OK;
   if (!indices || (num_keys > 0 && !scores)) return SAS_ERR_INVALID;
-  if (rows > INT32_MAX / 8) return SAS_ERR_UNSUPPORTED;
+  // Positions and outputs are stepped through by up to a cluster's threads.
+  if (rows > INT32_MAX / 8 || topk > SAS_MAX_TOPK || num_keys > INT32_MAX - 65536)
+    return SAS_ERR_UNSUPPORTED;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   // The smallest block whose registers hold the row, or a cluster of as few of
   // the largest as it takes (a cluster's barriers and remote reads cost more

@@ -83,10 +83,12 @@ def _index_params(q, weights, key_pool, block_table, cu_seqlens_q, seqused_kv, c
         raise ValueError("seqused_kv must have one entry per sequence")
     if weights.device != dev or key_pool.device != dev:
         raise ValueError("weights and key_pool must be on q's device")
-    if cmp_ratio < 1:
+    if not 1 <= cmp_ratio <= _lib.INT32_MAX:
         raise ValueError(f"cmp_ratio must be >= 1 (got {cmp_ratio})")
+    if total > _lib.INT32_MAX:
+        raise ValueError(f"q holds more than 2^31 - 1 tokens ({total})")
     N = table_shape[1] * pool_shape[1] if max_keys is None else int(max_keys)
-    if not 0 <= N <= 2 ** 31 - 1024:
+    if not 0 <= N <= _lib.INT32_MAX - 65536:
         raise ValueError(f"max_keys out of range ({N})")
     qf, w, pool = q.contiguous(), weights.contiguous(), key_pool.contiguous()
     if (qf.data_ptr() | pool.data_ptr()) & 15:
@@ -171,12 +173,12 @@ def select_topk(scores: torch.Tensor, topk: int, *,
     shape, topk = scores.shape, int(topk)
     if scores.dtype is not torch.float32 or len(shape) not in (2, 3):
         raise ValueError("scores must be float32 [T, N] or [B, S, N]")
-    if topk < 1:
-        raise ValueError(f"topk must be >= 1 (got {topk})")
+    if not 1 <= topk <= _lib.SAS_MAX_TOPK:
+        raise ValueError(f"topk must be in [1, 2^30] (got {topk})")
     N = shape[-1]
     rows = shape[0] if len(shape) == 2 else shape[0] * shape[1]
-    if rows > (2 ** 31 - 1) // 8:
-        raise ValueError("scores hold more than 2^28 - 1 rows")
+    if rows > _lib.INT32_MAX // 8 or N > _lib.INT32_MAX - 65536:
+        raise ValueError(f"scores hold too many rows or columns ({rows} x {N})")
     out = scores.new_empty((*shape[:-1], 1, topk), dtype=torch.int32)
     if lengths is not None:
         if lengths.numel() != rows:
@@ -209,8 +211,8 @@ def select_keys(q: torch.Tensor, weights: torch.Tensor, *, key_pool: torch.Tenso
     p, N, keep = _index_params(q, weights, key_pool, block_table, cu_seqlens_q, seqused_kv,
                                cmp_ratio, layout_q, max_keys)
     topk = int(topk)
-    if topk < 1:
-        raise ValueError(f"topk must be >= 1 (got {topk})")
+    if not 1 <= topk <= _lib.SAS_MAX_TOPK:
+        raise ValueError(f"topk must be in [1, 2^30] (got {topk})")
     dev, total = q.device, p.total_tokens
     out = torch.empty((*q.shape[:-2], 1, topk), dtype=torch.int32, device=dev)
     if total == 0:

@@ -109,8 +109,10 @@ def append_paged_kv_norm_rope(kv_pool: torch.Tensor, block_table: torch.Tensor,
     table_shape = block_table.shape
     if len(table_shape) != 2 or table_shape[0] < 1:
         raise ValueError("block_table must be [B, table_len] with B >= 1")
-    if cmp_ratio < 1:
+    if not 1 <= cmp_ratio <= _lib.INT32_MAX:
         raise ValueError(f"cmp_ratio must be >= 1 (got {cmp_ratio})")
+    if max(new_rows.numel() // D, pool_shape[0], pool_shape[1]) > _lib.INT32_MAX:
+        raise ValueError("more than 2^31 - 1 rows or blocks")
     B = table_shape[0]
     if cu_seqlens_new.numel() != B + 1 or start_pos.numel() != B:
         raise ValueError("cu_seqlens_new must have B + 1 entries and start_pos B")

@@ -44,7 +44,9 @@ def row_transform(dtype, device, head_dim, cos, sin, norm_dim, norm_weight, eps,
         shape = cos.shape
         if len(shape) != 2 or shape != sin.shape:
             raise ValueError("cos and sin must be [positions, rope_dim / 2]")
-        rows, rope_dim = min(shape[0], 2 ** 31 - 1), 2 * shape[1]
+        rows, rope_dim = min(shape[0], _lib.INT32_MAX), 2 * shape[1]
+        if rows < 1:
+            raise ValueError("cos and sin hold no position")
         if rope_dim % 16 or not 16 <= rope_dim <= min(head_dim, _lib.SAS_MAX_ROPE_DIM):
             raise ValueError(f"rope_dim must be a multiple of 16 up to "
                              f"{min(head_dim, _lib.SAS_MAX_ROPE_DIM)} (got {rope_dim})")

@@ -125,6 +125,12 @@ def test_entry_points_refuse_without_a_launch():
         assert topk(**bad) == 1, bad
 
 
+def test_topk_entry_refuses_sizes_past_32_bits():
+    L = _lib.lib()
+    for rows, n, k in ((1, 8, 2 ** 30 + 1), (2 ** 28, 8, 4), (1, 2 ** 31 - 1, 4)):
+        assert L.sas_topk_select(16, n, None, rows, n, k, 16, None) == 2, (rows, n, k)
+
+
 # ---- on a GPU: scores ----
 
 def score_case(seed, q_lens, kv, H, D, bs, ratio=1, dtype=torch.bfloat16, cols=None, spare=3):
@@ -377,6 +383,29 @@ def test_gpu_refusals():
              "cu_seqlens_q": torch.tensor([0, 0]).cuda()}
     assert indexer.index_scores(**empty).shape[0] == 0
     assert indexer.select_keys(topk=3, **empty).shape == (0, 1, 3)
+
+
+@pytest.mark.gpu
+def test_gpu_sizes_at_their_ends():
+    case = score_case(13, (2,), (50,), 4, 64, 16)
+    q, w, pool, table, cu, kv, _, N = case
+    good = dict(q=q.cuda(), weights=w.cuda(), key_pool=pool.cuda(), block_table=table.cuda(),
+                cu_seqlens_q=torch.tensor(cu).cuda(), seqused_kv=torch.tensor(kv).cuda())
+    x = torch.zeros(3, 8).cuda()
+    for k in (-1, 2 ** 30 + 1, 2 ** 32 + 2):
+        with pytest.raises(ValueError, match="topk"):
+            indexer.select_topk(x, k)
+        with pytest.raises(ValueError, match="topk"):
+            indexer.select_keys(topk=k, **good)
+    with pytest.raises(ValueError, match="ratio"):
+        indexer.index_scores(**{**good, "cmp_ratio": 2 ** 32 + 1})
+    # No columns, no pages, no pool.
+    s, n = indexer.index_scores(max_keys=0, return_lengths=True, **good)
+    assert s.shape == (2, 0) and n.tolist() == [0, 0]
+    for change in (dict(block_table=table.cuda()[:, :0]), dict(key_pool=pool.cuda()[:0])):
+        s, n = indexer.index_scores(max_keys=9, return_lengths=True, **{**good, **change})
+        assert bool((s == NEG).all()) and s.shape == (2, 9) and n.tolist() == [9, 9]
+        assert bool((indexer.select_keys(topk=3, max_keys=9, **{**good, **change}) == -1).all())
 
 
 # ---- on a GPU: selection ----

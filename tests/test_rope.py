@@ -86,6 +86,13 @@ def test_transform_refuses(change, word):
         row_transform(**kw)
 
 
+def test_transform_refuses_empty_tables():
+    none = torch.zeros(0, 32)
+    with pytest.raises(ValueError, match="no position"):
+        row_transform(torch.bfloat16, torch.device("cpu"), 576, none, none, 512, None, EPS, True,
+                      False)
+
+
 def test_entry_points_refuse_without_a_launch():
     from sparse_attn_sharedkv_b200.kv_cache import append_paged_kv_norm_rope
     from sparse_attn_sharedkv_b200.rope import norm_rope
@@ -184,6 +191,30 @@ def test_gpu_norm_rope(D, rope, norm, wt, inter, dtype):
         if rope:
             want, mag = reference(x, pos[:, None].expand(T, H), cos, sin, norm, w, inter, True)
             check(norm_rope(x, pos, cos, sin, inverse=True, **kw), want, mag, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D, rope, norm, wt, inter", [
+    *[ROWS[i] for i in (0, 1, 2, 3, 6, 8, 10, 11)],
+    (576, 256, 576, torch.float32, True), (576, 256, 576, "row", False),
+    (320, 144, 200, torch.float32, True), (1024, 256, 512, None, False)])
+def test_gpu_norm_rope_many_rows_and_wide_rotations(D, rope, norm, wt, inter):
+    # 12000 rows: more than all blocks that are resident at once take in one step.
+    from sparse_attn_sharedkv_b200.rope import norm_rope
+    for T, H in ((300, 40), (3, 5)):
+        x, cos, sin, w, _ = row_case(D, rope, norm, wt, torch.bfloat16, T * H, D + rope)
+        x = x.view(T, H, D)
+        pos = torch.randint(0, 4096, (T,), generator=torch.Generator().manual_seed(T)).cuda()
+        kw = dict(norm_dim=norm, norm_weight=w, eps=EPS, interleaved=inter)
+        want, mag = reference(x, pos[:, None].expand(T, H), cos, sin, norm, w, inter)
+        y = norm_rope(x, pos, cos, sin, **kw)
+        check(y, want, mag, torch.bfloat16)
+        bad = torch.arange(T, device="cuda") % 7 == 2  # rows outside the tables, between others
+        z = x.clone()
+        norm_rope(z, torch.where(bad, 4096 - 8191 * (pos % 2), pos), cos, sin, out=z, **kw)
+        if rope:
+            y[bad] = 0
+        assert torch.equal(z, y)
 
 
 @pytest.mark.gpu
