@@ -335,6 +335,10 @@ struct AppendArgs {
   int32_t num_blocks, block_size, table_len, batch, total, ratio;
 };
 
+// One row for each eight lanes.  Few rows are a chain of latencies (the search's
+// probes, the page, the row): the row itself is asked for first.  8 x 4096 rows
+// of 576 columns take 25 us, twice what their bytes need: 3.5 rounds of such
+// chains.
 template <int V, bool kBf16, Weights kW>
 __global__ void __launch_bounds__(kThreads, 2)
     append_norm_rope_kernel(RowArgs a, AppendArgs p) {

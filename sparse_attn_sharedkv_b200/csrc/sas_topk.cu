@@ -4,7 +4,7 @@
 // (golden.py:28-66 stops at the first -1).  A score of -inf is never
 // selected; NaN ranks above +inf and -0 equals +0.
 //
-// A row is read once and stays in the registers of a block, 16 scores a
+// A row is read once and stays in the registers of a block, 16 or 32 scores a
 // thread, or of a cluster of up to 8 blocks that exchange a few values through
 // distributed shared memory.  Rows of finite scores (the ordinary case):
 //
@@ -16,8 +16,8 @@
 //   3. scores in higher bins are selected, those of the border bin listed (if
 //      they are more than 512, those of one bin of a second histogram inside
 //      of it);
-//   4. among more than 32 listed, a histogram inside of the bin again; the
-//      border ones left are ranked by (score, position), and the list's
+//   4. up to 32 listed are ranked by (score, position) by the threads that hold
+//      them; among more, a histogram inside of the bin again, and the list's
 //      winners are marked for the threads that hold them;
 //   5. the selected positions are counted and written.
 //
@@ -29,9 +29,14 @@
 //
 // Each warp of a block holds neighbouring positions, 32 a round: loads are
 // coalesced for any row alignment, the count of the selected positions before
-// a warp's is one number, and the selected lanes of a round write neighbouring
-// words.  The flags of four rounds are four bytes of a word, so one shuffle
-// scan counts them.
+// a warp's is one number, a ballot counts those of a round, and its selected
+// lanes write neighbouring words.
+//
+// The floor is one read of the scores and one write of the positions; what
+// bounds many rows is the issue of instructions (70 % of the slots; about 60 a
+// score of a lane) with the latency of the phases.  32768 causal rows of up to
+// 4096, K 2048: 178 us (82 us of memory); 4000 rows of 16384 to 32768: 230 us; 64
+// rows of 8192 to 32768: 12 us.
 
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -44,7 +49,8 @@ namespace {
 
 constexpr int kBins = 1024;
 constexpr int kCand = 512;                 // border scores listed
-constexpr int kList = 128;                 // keys ranked directly
+constexpr int kList = 128;                 // keys ranked by as many threads
+constexpr int kDirect = 32;                // entries ranked by the threads that list them
 constexpr uint32_t kNegInf = 0x007fffffu;  // key of -inf
 constexpr uint32_t kPosInf = 0xff800000u;  // key of +inf
 
@@ -52,6 +58,11 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   if (x != x) return 0xffffffffu;
   const uint32_t u = __float_as_uint(x + 0.0f);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+// A score's key and its position as one number: greater is selected first.
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t pos) {
+  return (uint64_t)key << 32 | (uint32_t)~pos;
 }
 
 __device__ __forceinline__ float score_of(uint32_t key) {
@@ -73,6 +84,14 @@ __device__ __forceinline__ uint32_t peer_load(const void* p, int rank) {
 }
 __device__ __forceinline__ void peer_store(void* p, int rank, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_smem(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint64_t peer_load64(const void* p, int rank) {
+  uint64_t v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer_smem(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void peer_store64(void* p, int rank, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_smem(p, rank)), "l"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t peer_add(void* p, int rank, uint32_t v) {
   uint32_t old;
@@ -101,12 +120,22 @@ struct TopkShared {
   uint32_t rmin[C], rmax[C], rcnt[C], rtot[C];  // one entry per block of the cluster
   uint32_t bin, above, inside;                  // found in the histogram, bin from the top
   uint32_t listed, ranked;
-  uint32_t list_key[kCand], list_pos[kCand];            // of the cluster, in block 0
-  uint32_t mine_key[C > 1 ? kCand : 1], mine_pos[C > 1 ? kCand : 1];  // own copy
-  uint32_t key[kList], pos[kList];
+  alignas(16) uint64_t list[kCand];        // of the cluster, in block 0
+  alignas(16) uint64_t mine[C > 1 ? kCand : 2];  // own copy
+  uint64_t entry[kList];
   uint32_t taken[T];  // listed scores of each thread that are selected
-  uint32_t thr_key, thr_pos;
+  uint64_t threshold;
 };
+
+// One more entry of the row's list.
+template <int T, int C>
+__device__ __forceinline__ void add_entry(TopkShared<T, C>& s, uint64_t e) {
+  if constexpr (C == 1) {
+    s.list[atomicAdd(&s.listed, 1u)] = e;
+  } else {
+    peer_store64(&s.list[peer_add(&s.listed, 0, 1u)], 0, e);
+  }
+}
 
 // Positions of a block: `len` from `begin` on, `seg` for each warp.
 struct Places {
@@ -210,35 +239,14 @@ __device__ __forceinline__ void find_bin(TopkShared<T, C>& s, uint32_t need) {
   __syncthreads();
 }
 
-// Count, over the row's positions, of the flags (bit i: the thread's position
-// of round i, none behind round `last`) before each of the thread's positions:
-// the returned count, of the warps and blocks before, and at[i] for round i.
-template <int T, int C, int P>
-__device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, uint32_t flags,
-                                                 int last, uint32_t (&at)[P]) {
+// Count of the flags set in the row's warps and blocks before this warp.  The
+// flags of its own rounds are then counted by ballots.
+template <int T, int C>
+__device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, uint32_t flags) {
   constexpr int W = T / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t sum = 0;  // of the warp's rounds so far
-#pragma unroll
-  for (int g = 0; g < P / 4; ++g) {
-    if (4 * g > last) break;
-    // Bits 0 .. 3 of the group into the low bits of four bytes.
-    const uint32_t own = ((flags >> (4 * g) & 15u) * 0x00204081u) & 0x01010101u;
-    uint32_t v = own;  // at most 32 in each byte
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += up;
-    }
-    // Bytes of the rounds before in the group; all stay below 128.
-    const uint32_t total = __shfl_sync(0xffffffffu, v, 31);
-    v += total * 0x01010100u - own;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) at[4 * g + k] = sum + ((v >> (8 * k)) & 255u);
-    sum += (total * 0x01010101u) >> 24;
-  }
-  __syncthreads();
-  if (lane == 0) s.wsum[warp] = sum;
+  const uint32_t own = __reduce_add_sync(0xffffffffu, __popc(flags));
+  if (lane == 0) s.wsum[warp] = own;
   __syncthreads();
   const uint32_t other = lane < W ? s.wsum[lane] : 0u;
   uint32_t base = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0u);
@@ -351,55 +359,38 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       sel |= cand;
     } else if (equal) {
       // The first `need` of the equal keys by position.
-      uint32_t at[P];
-      const uint32_t base = count_before<T, C>(s, rank, cand, P - 1, at);
+      uint32_t base = count_before<T, C>(s, rank, cand);
+      const uint32_t below = (1u << (tid & 31)) - 1u;
 #pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (cand >> i & 1) sel |= (base + at[i] < need ? 1u : 0u) << i;
+      for (int i = 0; i < P; ++i) {
+        const uint32_t on = __ballot_sync(0xffffffffu, cand >> i & 1);
+        if (cand >> i & 1) sel |= (base + __popc(on & below) < need ? 1u : 0u) << i;
+        base += __popc(on);
+      }
       row_sync<C>();  // before the counts are written again
     } else {
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        if (cand >> i & 1) {
-          const uint32_t p = (uint32_t)pl.at(i);
-          if constexpr (C == 1) {
-            const uint32_t l = atomicAdd(&s.listed, 1u);
-            s.key[l] = key[i];
-            s.pos[l] = p;
-          } else {
-            const uint32_t l = peer_add(&s.listed, 0, 1u);
-            peer_store(&s.list_key[l], 0, key[i]);
-            peer_store(&s.list_pos[l], 0, p);
-          }
-        }
-      }
+      for (int i = 0; i < P; ++i)
+        if (cand >> i & 1) add_entry<T, C>(s, entry_of(key[i], (uint32_t)pl.at(i)));
       row_sync<C>();
+      const uint64_t* list = s.list;
       if constexpr (C > 1) {
-        if (tid < (int)inside) {
-          s.key[tid] = peer_load(&s.list_key[tid], 0);
-          s.pos[tid] = peer_load(&s.list_pos[tid], 0);
-        }
+        if (tid < (int)inside) s.mine[tid] = peer_load64(&s.list[tid], 0);
         __syncthreads();
+        list = s.mine;
       }
       if (tid < (int)inside) {
-        const uint32_t k = s.key[tid], p = s.pos[tid];
+        const uint64_t e = list[tid];
         uint32_t r = 0;
-        for (int j = 0; j < (int)inside; ++j)
-          r += s.key[j] > k || (s.key[j] == k && s.pos[j] < p) ? 1u : 0u;
-        if (r + 1 == need) {
-          s.thr_key = k;
-          s.thr_pos = p;
-        }
+        for (int j = 0; j < (int)inside; ++j) r += list[j] > e ? 1u : 0u;
+        if (r + 1 == need) s.threshold = e;
       }
       __syncthreads();
-      const uint32_t tk = s.thr_key, tp = s.thr_pos;
+      const uint64_t threshold = s.threshold;
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        if (cand >> i & 1) {
-          const uint32_t p = (uint32_t)pl.at(i);
-          sel |= (key[i] > tk || (key[i] == tk && p <= tp) ? 1u : 0u) << i;
-        }
-      }
+      for (int i = 0; i < P; ++i)
+        if (cand >> i & 1)
+          sel |= (entry_of(key[i], (uint32_t)pl.at(i)) >= threshold ? 1u : 0u) << i;
     }
   }
 
@@ -429,15 +420,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// One block a row: as many blocks as the SM has threads for (32 registers, a
-// few of them spilled), since a row is a chain of short phases: 32768 rows of up
-// to 4096 take 214 us so, 251 us at 1280 threads an SM without spills.
+// Rounds a thread: 32 make the barriers and scans of a row cheaper by half, 16
+// make its phases shorter (launcher).  1024 threads an SM, 64 registers each:
+// 30000 rows of 1500 to 2048, K 512, take 137 us so, 174 us with 2048 threads of
+// 32 registers, some of them spilled.
 template <int T, int C, int P>
-__global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster_dims__(C, 1, 1)
+__global__ void __launch_bounds__(T, C == 1 ? 1024 / T : 1) __cluster_dims__(C, 1, 1)
     topk_kernel(const float* __restrict__ scores, int64_t stride,
-                const int32_t* __restrict__ lengths, int n_cols, int K,
+                const int32_t* __restrict__ lengths, int rows, int ahead, int n_cols, int K,
                 int32_t* __restrict__ out) {
   constexpr int W = T / 32;
+  constexpr int kStep = 4;  // rounds between looks at the last one
   constexpr float kShift = 8388608.0f;         // 2^23: integers are its low bits
   constexpr uint32_t kShiftBits = 0x4b000000u;
   __shared__ TopkShared<T, C> s;
@@ -463,8 +456,16 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
   float low = first, high = first;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    if (i > last) break;
+    if (i % kStep == 0 && i > last) break;
     v[i] = i < rounds ? __ldg(x + pl.at(i)) : first;
+  }
+  // The row that a later block will take comes into L2 meanwhile.
+  if (C == 1 && row + ahead < rows) {
+    int m = n_cols;
+    if (lengths != nullptr) m = min(m, __ldg(lengths + row + ahead));
+    const float* y = x + ahead * stride;
+    for (int c = tid * 32; c < m; c += T * 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(y + c));
   }
   const bool short_row = n <= K;
   if (short_row) {
@@ -474,12 +475,12 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
     for (int i = n + rank * T + tid; i < K; i += C * T) o[i] = -1;
   } else {
     clear_histogram<T, C>(s);
-    s.taken[tid] = 0;
-    if (tid == 0) s.listed = s.ranked = 0;
+    if (tid < kDirect + 4) s.list[tid] = 0;
+    if (tid == 0) s.listed = 0;
   }
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    if (i > last) break;
+    if (i % kStep == 0 && i > last) break;
     low = min_nan(low, v[i]);
     high = max_nan(high, v[i]);
   }
@@ -514,7 +515,7 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
     auto place = [&](float a) { return fmaf(a - low, scale, kShift); };
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      if (i > last) break;
+      if (i % kStep == 0 && i > last) break;
       if (i < rounds)
         atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place(v[i]))], 1u);
     }
@@ -537,7 +538,7 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        if (i > last) break;
+        if (i % kStep == 0 && i > last) break;
         if (i < rounds && place(v[i]) == bin)
           atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place2(v[i]))], 1u);
       }
@@ -549,52 +550,34 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
     if (inside == need || inside <= kCand) {
       const bool all = inside == need;
       uint32_t cand = 0;  // of the border
+      float border = 0.0f;  // the score of its highest bit
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        if (i > last) break;
+        if (i % kStep == 0 && i > last) break;
         const float t = place(v[i]);
         sel |= (t > bin ? 1u : 0u) << i;
         cand |= (t == bin ? 1u : 0u) << i;
+        if (t == bin) border = v[i];
       }
       const uint32_t valid = rounds < 32 ? (1u << rounds) - 1u : 0xffffffffu;
+      const int kept = cand > valid ? -1 : 31 - __clz(cand);  // the bit `border` belongs to
       sel &= valid;
       cand &= valid;
+      auto score_at = [&](int i) { return i == kept ? border : __ldg(x + pl.at(i)); };
+      uint32_t mine = 0;  // listed of this thread
       if (twice || !all) {
-        // Few of the border a thread: looked at one by one, read again.
-        const int count = __popc(cand);
-        uint32_t slot = 0;
-        if (!twice) {
-          // A place for each in the list.
-          uint32_t incl = (uint32_t)count;
-#pragma unroll
-          for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += up;
-          }
-          if (lane == 31 && incl > 0)
-            slot = C == 1 ? atomicAdd(&s.listed, incl) : peer_add(&s.listed, 0, incl);
-          slot = __shfl_sync(0xffffffffu, slot, 31) + incl - (uint32_t)count;
-        }
-        for (uint32_t rest = cand; rest != 0; rest &= rest - 1) {
-          const int i = __ffs(rest) - 1;
-          const uint32_t p = (uint32_t)pl.at(i);
-          const float a = __ldg(x + p);
+        // Few of the border a thread, most often one.
+        for (uint32_t rest = cand; rest != 0;) {
+          const int i = 31 - __clz(rest);
+          rest ^= 1u << i;
+          const float a = score_at(i);
           if (twice) {
             const float d = place2(a) - bin2;
             if (d > 0.0f || (all && d == 0.0f)) sel |= 1u << i;
             if (d != 0.0f || all) continue;
-            slot = C == 1 ? atomicAdd(&s.listed, 1u) : peer_add(&s.listed, 0, 1u);
           }
-          // -0 as +0, so that words of equal scores are equal.
-          const uint32_t word = __float_as_uint(a + 0.0f);
-          if constexpr (C == 1) {
-            s.list_key[slot] = word;
-            s.list_pos[slot] = p;
-          } else {
-            peer_store(&s.list_key[slot], 0, word);
-            peer_store(&s.list_pos[slot], 0, p);
-          }
-          ++slot;
+          mine |= 1u << i;
+          add_entry<T, C>(s, entry_of(key_of(a), (uint32_t)pl.at(i)));
         }
       } else {
         sel |= cand;
@@ -602,72 +585,75 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
       general = false;
       if (!all) {
         row_sync<C>();
-        const uint32_t* keys = s.list_key;
-        const uint32_t* poss = s.list_pos;
+        const uint64_t* list = s.list;
         if constexpr (C > 1) {
-          for (int i = tid; i < (int)inside; i += T) {
-            s.mine_key[i] = peer_load(&s.list_key[i], 0);
-            s.mine_pos[i] = peer_load(&s.list_pos[i], 0);
-          }
-          keys = s.mine_key;
-          poss = s.mine_pos;
+          for (int i = tid; i < min((int)inside + 3, kCand); i += T)
+            s.mine[i] = peer_load64(&s.list[i], 0);
+          list = s.mine;
         }
-        // What the list's entries are told apart by: their bin inside of the
-        // border bin (or of bin2), then (score, position).
-        const float edge3 = twice ? bin2 - kShift - 0.5f : 0.0f;
-        auto place3 = [&](float a) {
-          const float u = fmaf(a - low, scale, -edge) * (float)kBins;
-          const float w = twice ? (u - edge3) * (float)kBins : u;
-          return fminf(fmaxf(w, 0.0f), (float)(kBins - 1)) + kShift;
-        };
-        float bin3 = 0.0f;  // every entry's bin is above it
-        uint32_t left = inside;
-        const bool thrice = inside > 32;
-        if (thrice) {
+        if (inside <= kDirect) {
+          // Each thread ranks its own entries, four at a time against the list
+          // (zeros behind it).
+          if constexpr (C > 1) __syncthreads();
+          for (uint32_t rest = mine; rest != 0;) {
+            const int i = 31 - __clz(rest);
+            rest ^= 1u << i;
+            const uint64_t e = entry_of(key_of(score_at(i)), (uint32_t)pl.at(i));
+            uint32_t r = 0;
+            for (int j = 0; j < (int)inside; j += 4) {
+              const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(list + j);
+              const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(list + j + 2);
+              r += (a.x > e ? 1u : 0u) + (a.y > e ? 1u : 0u) + (b.x > e ? 1u : 0u) +
+                   (b.y > e ? 1u : 0u);
+            }
+            if (r < need) sel |= 1u << i;
+          }
+        } else {
+          // What the list's entries are told apart by: their bin inside of the
+          // border bin (or of bin2), then (score, position).
+          const float edge3 = twice ? bin2 - kShift - 0.5f : 0.0f;
+          auto place3 = [&](float a) {
+            const float u = fmaf(a - low, scale, -edge) * (float)kBins;
+            const float w = twice ? (u - edge3) * (float)kBins : u;
+            return fminf(fmaxf(w, 0.0f), (float)(kBins - 1)) + kShift;
+          };
           clear_histogram<T, C>(s);
+          s.taken[tid] = 0;
+          if (tid == 0) s.ranked = 0;
           __syncthreads();
           for (int i = tid; i < (int)inside; i += T)
             atomicAdd(&s.hist[kShiftBits + (kBins - 1) -
-                              __float_as_uint(place3(__uint_as_float(keys[i])))],
+                              __float_as_uint(place3(score_of((uint32_t)(list[i] >> 32))))],
                       1u);
           find_bin<T, C, true>(s, need);
-          bin3 = kShift + (float)(kBins - 1 - (int)s.bin);
+          const float bin3 = kShift + (float)(kBins - 1 - (int)s.bin);
           need -= s.above;
-          left = s.inside;
-        } else if constexpr (C > 1) {
-          __syncthreads();
-        }
-        if (left > kList) {
-          general = true;  // the same in every block of the row
-        } else {
-          auto take = [&](uint32_t p) {
-            if ((int)p < begin || (int)p >= end) return;
-            const int q = (int)p - begin, w = q / pl.seg, r = q - w * pl.seg;
-            atomicOr(&s.taken[w * 32 + (r & 31)], 1u << (r >> 5));
-          };
-          for (int i = tid; i < (int)inside; i += T) {
-            const float d = thrice ? place3(__uint_as_float(keys[i])) - bin3 : 0.0f;
-            if (d > 0.0f) {
-              take(poss[i]);
-            } else if (d == 0.0f) {
-              const uint32_t l = atomicAdd(&s.ranked, 1u);
-              s.key[l] = keys[i];
-              s.pos[l] = poss[i];
+          const uint32_t left = s.inside;
+          if (left > kList) {
+            general = true;  // the same in every block of the row
+          } else {
+            auto take = [&](uint32_t p) {
+              if ((int)p < begin || (int)p >= end) return;
+              const int q = (int)p - begin, w = q / pl.seg, r = q - w * pl.seg;
+              atomicOr(&s.taken[w * 32 + (r & 31)], 1u << (r >> 5));
+            };
+            for (int i = tid; i < (int)inside; i += T) {
+              const float d = place3(score_of((uint32_t)(list[i] >> 32))) - bin3;
+              if (d > 0.0f)
+                take(~(uint32_t)list[i]);
+              else if (d == 0.0f)
+                s.entry[atomicAdd(&s.ranked, 1u)] = list[i];
             }
-          }
-          __syncthreads();
-          if (tid < (int)left) {
-            const float a = __uint_as_float(s.key[tid]);
-            const uint32_t p = s.pos[tid];
-            uint32_t r = 0;
-            for (int j = 0; j < (int)left; ++j) {
-              const float b = __uint_as_float(s.key[j]);
-              r += b > a || (b == a && s.pos[j] < p) ? 1u : 0u;
+            __syncthreads();
+            if (tid < (int)left) {
+              const uint64_t e = s.entry[tid];
+              uint32_t r = 0;
+              for (int j = 0; j < (int)left; ++j) r += s.entry[j] > e ? 1u : 0u;
+              if (r < need) take(~(uint32_t)e);
             }
-            if (r < need) take(p);
+            __syncthreads();
+            sel |= s.taken[tid];
           }
-          __syncthreads();
-          sel |= s.taken[tid];
         }
       }
     }
@@ -678,12 +664,23 @@ __global__ void __launch_bounds__(T, C == 1 && P == 16 ? 2048 / T : 1) __cluster
     sel = select_general<T, C, P>(s, x, pl, rank, K, &able);
   }
 
-  uint32_t at[P];
-  int32_t* dst = o + count_before<T, C>(s, rank, sel, last, at);
+  uint32_t base = count_before<T, C>(s, rank, sel);
+  const uint32_t below = (1u << lane) - 1u;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    if (i > last) break;
-    if (sel >> i & 1) dst[at[i]] = pl.at(i);
+    if (i % kStep == 0 && i > last) break;
+    uint32_t on;  // written out, for one predicate and no branch
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 c;\n\t.reg .b64 a;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "vote.sync.ballot.b32 %0, p, 0xffffffff;\n\t"
+        "and.b32 c, %0, %2;\n\tpopc.b32 c, c;\n\tadd.u32 c, c, %3;\n\t"
+        "mad.wide.u32 a, c, 4, %4;\n\t"
+        "@p st.global.u32 [a], %5;\n\t}"
+        : "=&r"(on)
+        : "r"(sel & (1u << i)), "r"(below), "r"(base), "l"(o), "r"(pl.at(i))
+        : "memory");
+    base += __popc(on);
   }
   const uint32_t filled = min(able, (uint32_t)K);
   for (uint32_t i = filled + rank * T + tid; i < (uint32_t)K; i += C * T) o[i] = -1;
@@ -783,19 +780,26 @@ extern "C" int sas_topk_select(const float* scores, int64_t score_stride, const 
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   // The smallest block whose registers hold the row, or a cluster of as few of
   // the largest as it takes (a cluster's barriers and remote reads cost more
-  // than a block's longer phases: 256 rows of 32768 take 29 us in blocks of 1024
-  // threads and 86 us in clusters of four of 512) unless the rows are so few
-  // that the clusters fit the SMs side by side.
+  // than a block's longer phases: 256 rows of 32768 take 23 us in blocks of 1024
+  // threads and 63 us in clusters of four of 512) unless the rows are so few
+  // that the clusters fit the SMs side by side (16 rows 10.3 against 12.3 us).  Rows of up to 16384 take 32
+  // scores a thread where there are many of them: 4000 rows of 4096 to 8192 62 us
+  // (73 us with 16 a thread), 32768 of up to 4096 178 (197), but 8 rows of 4096
+  // 10.3 us (8.2); about 300 to 600 rows take the same time either way.
 #define SAS_TOPK(T, C, P)                                                                          \
-  topk_kernel<T, C, P><<<(unsigned)rows * C, T, 0, stream>>>(scores, score_stride, lengths,        \
-                                                             num_keys, topk, indices)
+  topk_kernel<T, C, P><<<(unsigned)rows * C, T, 0, stream>>>(                                     \
+      scores, score_stride, lengths, rows, sms * (1024 / T), num_keys, topk, indices)
   int dev = 0;
   const int sms = sas::current_device_sms(&dev);
   if (sms <= 0) return SAS_ERR_CUDA;
   const bool few = (int64_t)rows * 4 <= sms;
+  const bool many = rows > 2 * sms;
   if (num_keys <= 16 * 128) SAS_TOPK(128, 1, 16);
+  else if (num_keys <= 32 * 128 && many) SAS_TOPK(128, 1, 32);
   else if (num_keys <= 16 * 256) SAS_TOPK(256, 1, 16);
+  else if (num_keys <= 32 * 256 && many) SAS_TOPK(256, 1, 32);
   else if (num_keys <= 16 * 512) SAS_TOPK(512, 1, 16);
+  else if (num_keys <= 32 * 512 && many) SAS_TOPK(512, 1, 32);
   else if (num_keys <= 16 * 1024) SAS_TOPK(1024, 1, 16);
   else if (num_keys <= 32 * 1024 && few) SAS_TOPK(512, 4, 16);
   else if (num_keys <= 32 * 1024) SAS_TOPK(1024, 1, 32);

@@ -469,6 +469,21 @@ def test_gpu_select_topk(rows, N, K, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows, N, K", [(310, 3001, 1500), (300, 6007, 512), (299, 16000, 2048)])
+def test_gpu_select_topk_many_rows(rows, N, K, kind):
+    # More than two rows for each SM, of which some are empty, shorter than K or whole.
+    g = torch.Generator().manual_seed(N + K)
+    x = topk_rows(kind, rows, N, g)
+    lengths = torch.randint(0, N + 1, (rows,), generator=g, dtype=torch.int32)
+    lengths[:6] = torch.tensor([0, N, 1, K, K + 1, N])
+    d = x.cuda()
+    got = indexer.select_topk(d, K, lengths=lengths.cuda())
+    assert np.array_equal(got[:, 0].cpu().numpy(), topk_reference(x, K, lengths))
+    assert torch.equal(indexer.select_topk(d, K, lengths=lengths.cuda()), got)
+
+
+@pytest.mark.gpu
 def test_gpu_select_topk_strides_lengths_and_stream():
     g = torch.Generator().manual_seed(3)
     x = torch.randn(6, 1003, generator=g)
