@@ -5,7 +5,7 @@
 // selected; NaN ranks above +inf and -0 equals +0.
 //
 // A row is read once and stays in the registers of a block, 16 or 32 scores a
-// thread, or of a cluster of up to 8 blocks that exchange a few values through
+// thread, or of a cluster of up to 8 blocks (262144 scores) that exchange a few values through
 // distributed shared memory.  Rows of finite scores (the ordinary case):
 //
 //   1. the least and the greatest score; a row of at most K is all selected;
@@ -239,13 +239,12 @@ __device__ __forceinline__ void find_bin(TopkShared<T, C>& s, uint32_t need) {
   __syncthreads();
 }
 
-// Count of the flags set in the row's warps and blocks before this warp.  The
-// flags of its own rounds are then counted by ballots.
+// Sum of the threads' counts over the row's warps and blocks before this warp.
 template <int T, int C>
-__device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, uint32_t flags) {
+__device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, uint32_t count) {
   constexpr int W = T / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t own = __reduce_add_sync(0xffffffffu, __popc(flags));
+  const uint32_t own = __reduce_add_sync(0xffffffffu, count);
   if (lane == 0) s.wsum[warp] = own;
   __syncthreads();
   const uint32_t other = lane < W ? s.wsum[lane] : 0u;
@@ -257,6 +256,46 @@ __device__ __forceinline__ uint32_t count_before(TopkShared<T, C>& s, int rank, 
     base += __reduce_add_sync(0xffffffffu, lane < rank ? s.rtot[lane] : 0u);
   }
   return base;
+}
+
+// Bins linear in the scores for keys of -inf < score < +inf between the keys kmin
+// and kmax, +inf and NaN above.  A range whose scale is not finite (it overflows,
+// is subnormal or a single value) puts every finite score into the last bin.
+struct LinearBins {
+  float low, scale;
+
+  __device__ __forceinline__ LinearBins(uint32_t kmin, uint32_t kmax) : low(score_of(kmin)) {
+    scale = kmin <= kmax ? __fdividef(kBins - 0.5f, score_of(kmax) - low) : 0.0f;
+    if (!(scale < CUDART_INF_F)) scale = 0.0f;
+  }
+  __device__ __forceinline__ int operator()(uint32_t k) const {
+    if (k >= kPosInf) return 0;
+    // An infinite difference times a scale of zero is NaN, which max takes to 0.
+    return kBins - 1 - (int)fminf(fmaxf((score_of(k) - low) * scale, 0.0f), (float)(kBins - 1));
+  }
+};
+
+// The need-th greatest entry of the row's list of `inside` <= kList entries, in
+// every thread.
+template <int T, int C>
+__device__ __forceinline__ uint64_t list_threshold(TopkShared<T, C>& s, uint32_t inside,
+                                                   uint32_t need) {
+  const int tid = threadIdx.x;
+  row_sync<C>();
+  const uint64_t* list = s.list;
+  if constexpr (C > 1) {
+    if (tid < (int)inside) s.mine[tid] = peer_load64(&s.list[tid], 0);
+    __syncthreads();
+    list = s.mine;
+  }
+  if (tid < (int)inside) {
+    const uint64_t e = list[tid];
+    uint32_t r = 0;
+    for (int j = 0; j < (int)inside; ++j) r += list[j] > e ? 1u : 0u;
+    if (r + 1 == need) s.threshold = e;
+  }
+  __syncthreads();
+  return s.threshold;
 }
 
 // Selection flags of any row, by keys.  Shared memory is in use up to here by
@@ -290,16 +329,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
 #pragma unroll
     for (int i = 0; i < P; ++i) sel |= (key[i] > kNegInf ? 1u : 0u) << i;
   } else {
-    // Linear in the scores; a range whose scale is not finite (it overflows,
-    // is subnormal or a single value) puts every finite score into the last bin.
-    const float low = score_of(kmin);
-    float scale = kmin <= kmax ? __fdividef(kBins - 0.5f, score_of(kmax) - low) : 0.0f;
-    if (!(scale < CUDART_INF_F)) scale = 0.0f;
-    auto bin_of = [&](uint32_t k) {
-      if (k >= kPosInf) return 0;
-      // An infinite difference times a scale of zero is NaN, which max takes to 0.
-      return kBins - 1 - (int)fminf(fmaxf((score_of(k) - low) * scale, 0.0f), (float)(kBins - 1));
-    };
+    const LinearBins bin_of(kmin, kmax);
 #pragma unroll
     for (int i = 0; i < P; ++i)
       if (key[i] > kNegInf) atomicAdd(&s.hist[bin_of(key[i])], 1u);
@@ -359,7 +389,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
       sel |= cand;
     } else if (equal) {
       // The first `need` of the equal keys by position.
-      uint32_t base = count_before<T, C>(s, rank, cand);
+      uint32_t base = count_before<T, C>(s, rank, __popc(cand));
       const uint32_t below = (1u << (tid & 31)) - 1u;
 #pragma unroll
       for (int i = 0; i < P; ++i) {
@@ -372,21 +402,7 @@ __device__ __noinline__ uint32_t select_general(TopkShared<T, C>& s, const float
 #pragma unroll
       for (int i = 0; i < P; ++i)
         if (cand >> i & 1) add_entry<T, C>(s, entry_of(key[i], (uint32_t)pl.at(i)));
-      row_sync<C>();
-      const uint64_t* list = s.list;
-      if constexpr (C > 1) {
-        if (tid < (int)inside) s.mine[tid] = peer_load64(&s.list[tid], 0);
-        __syncthreads();
-        list = s.mine;
-      }
-      if (tid < (int)inside) {
-        const uint64_t e = list[tid];
-        uint32_t r = 0;
-        for (int j = 0; j < (int)inside; ++j) r += list[j] > e ? 1u : 0u;
-        if (r + 1 == need) s.threshold = e;
-      }
-      __syncthreads();
-      const uint64_t threshold = s.threshold;
+      const uint64_t threshold = list_threshold<T, C>(s, inside, need);
 #pragma unroll
       for (int i = 0; i < P; ++i)
         if (cand >> i & 1)
@@ -664,7 +680,7 @@ __global__ void __launch_bounds__(T, C == 1 ? 1024 / T : 1) __cluster_dims__(C, 
     sel = select_general<T, C, P>(s, x, pl, rank, K, &able);
   }
 
-  uint32_t base = count_before<T, C>(s, rank, sel);
+  uint32_t base = count_before<T, C>(s, rank, __popc(sel));
   const uint32_t below = (1u << lane) - 1u;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
@@ -687,83 +703,167 @@ __global__ void __launch_bounds__(T, C == 1 ? 1024 / T : 1) __cluster_dims__(C, 
   if constexpr (C > 1) row_sync<C>();  // no block leaves while another reads its shared memory
 }
 
-// Rows longer than a cluster holds: one block per row, the K-th largest key by
-// four passes of 8 bits over the row, then the positions above it and the
-// first ties by a scan over the row.
-constexpr int kLongThreads = 1024;
+// Rows longer than the registers of a cluster: a cluster of eight blocks reads its
+// row again for each step (from L2, after the first).  The border is a range of
+// keys that histograms narrow, first linear in the scores, then in the keys, and
+// the selected scores are the entries (key, position) from a threshold on.
+// One row of 1000000, K 2048, takes 100 us, 32 of them 300 us; 300 rows of 300000
+// 730 us.  (One block a row and four passes of 8 bits: 1020, 1660 and 930 us.)
+constexpr int kLongThreads = 1024, kLongBlocks = 8;
 
-__global__ void __launch_bounds__(kLongThreads)
+__global__ void __launch_bounds__(kLongThreads, 1) __cluster_dims__(kLongBlocks, 1, 1)
     topk_long_kernel(const float* __restrict__ scores, int64_t stride,
                      const int32_t* __restrict__ lengths, int n_cols, int K,
                      int32_t* __restrict__ out) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t sh_prefix, sh_need, sh_total;
-  __shared__ int warp_gt[kLongThreads / 32], warp_eq[kLongThreads / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x;
+  constexpr int T = kLongThreads, C = kLongBlocks;
+  __shared__ TopkShared<T, C> s;
+  const int tid = threadIdx.x, lane = tid & 31, rank = (int)(blockIdx.x % C);
+  const int64_t row = blockIdx.x / C;
   const float* x = scores + row * stride;
   int32_t* o = out + row * K;
   int n = n_cols;
-  if (lengths != nullptr) n = max(0, min(n, lengths[row]));
-  // Digits of the threshold key, from the top.
-  uint32_t prefix = 0, need = K;
-  bool all = false;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kLongThreads) hist[i] = 0;
-    if (tid == 0) sh_total = 0;
-    __syncthreads();
-    const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-    for (int64_t i = tid; i < n; i += kLongThreads) {
-      const uint32_t k = key_of(x[i]);
-      if (k > kNegInf && (k & high) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+  if (lengths != nullptr) n = max(0, min(n, __ldg(lengths + row)));
+  if (n == 0) {  // the whole row's blocks alike
+    for (int i = rank * T + tid; i < K; i += C * T) o[i] = -1;
+    return;
+  }
+  const int part = (int)(((int64_t)n + C - 1) / C);
+  const int begin = (int)min((int64_t)n, (int64_t)rank * part);
+  const Places pl(begin, min(n - begin, part) + begin, T);
+  const int rounds = pl.rounds();
+  // Eight rounds from `i` on, -inf behind the thread's last: loads first.
+  auto load = [&](int i, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = i + j < rounds ? __ldg(x + pl.at(i + j)) : -CUDART_INF_F;
+  };
+  auto each = [&](auto f) {
+    for (int i = 0; i < rounds; i += 8) {
+      float v[8];
+      load(i, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f(key_of(v[j]), pl.at(i + j));
     }
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t above = 0;
-      int d = 255;
-      for (; d >= 0; --d) {
-        if (above + hist[d] >= need) break;
-        above += hist[d];
+  };
+
+  clear_histogram<T, C>(s);
+  if (tid == 0) s.listed = 0;
+  uint32_t kmin = 0xffffffffu, kmax = 0, able = 0;
+  each([&](uint32_t k, int) {
+    able += k > kNegInf ? 1u : 0u;
+    if (k > kNegInf && k < kPosInf) {
+      kmin = min(kmin, k);
+      kmax = max(kmax, k);
+    }
+  });
+  uint32_t row_able = able;
+  row_reduce<T, C>(s, rank, kmin, kmax, row_able);
+
+  uint64_t threshold = (uint64_t)(kNegInf + 1) << 32;  // entries from it on are selected
+  uint32_t count = able;                               // selected ones of the thread
+  if (row_able > (uint32_t)K) {
+    uint32_t need = (uint32_t)K;
+    const LinearBins bin_of(kmin, kmax);
+    each([&](uint32_t k, int) {
+      if (k > kNegInf) atomicAdd(&s.hist[bin_of(k)], 1u);
+    });
+    find_bin<T, C>(s, need);
+    const int bin = (int)s.bin;
+    need -= s.above;
+    uint32_t inside = s.inside, none = 0;
+    count = 0;
+    if (inside <= kList) {
+      each([&](uint32_t k, int p) {
+        if (k <= kNegInf) return;
+        const int b = bin_of(k);
+        count += b < bin ? 1u : 0u;
+        if (b == bin) add_entry<T, C>(s, entry_of(k, (uint32_t)p));
+      });
+      threshold = list_threshold<T, C>(s, inside, need);
+    } else {
+      // The border's keys: its bin is a range of them.
+      uint32_t from = 0xffffffffu, to = 0;
+      each([&](uint32_t k, int) {
+        if (k > kNegInf && bin_of(k) == bin) {
+          from = min(from, k);
+          to = max(to, k);
+        }
+      });
+      row_reduce<T, C>(s, rank, from, to, none);
+      while (inside > need && inside > kList && from < to) {
+        // Every block has read the histograms: the barrier of row_reduce or the
+        // one below was behind them.
+        clear_histogram<T, C>(s);
+        __syncthreads();
+        const int shift = max(0, 22 - __clz(to - from));  // range >> shift below 1024
+        each([&](uint32_t k, int) {
+          if (k >= from && k <= to) atomicAdd(&s.hist[kBins - 1 - (int)((k - from) >> shift)], 1u);
+        });
+        find_bin<T, C>(s, need);
+        need -= s.above;
+        inside = s.inside;
+        from += (uint32_t)(kBins - 1 - (int)s.bin) << shift;
+        to = from + min(to - from, (1u << shift) - 1u);
+        row_sync<C>();
       }
-      sh_total = d < 0;
-      sh_prefix = prefix | ((uint32_t)max(d, 0) << shift);
-      sh_need = need - above;
+      const bool list = inside <= kList, all = inside == need;
+      uint32_t equal = 0;
+      each([&](uint32_t k, int p) {
+        count += k > to ? 1u : 0u;
+        if (k >= from && k <= to) {
+          ++equal;
+          if (list) add_entry<T, C>(s, entry_of(k, (uint32_t)p));
+        }
+      });
+      if (list) {
+        threshold = list_threshold<T, C>(s, inside, need);
+      } else if (all) {
+        threshold = (uint64_t)from << 32;
+        count += equal;
+      } else {
+        // Equal keys: the warp that holds the need-th of them looks for it.
+        uint32_t base = count_before<T, C>(s, rank, equal);
+        const uint32_t own = __reduce_add_sync(0xffffffffu, equal);
+        if (lane == 0) count += base < need ? min(own, need - base) : 0u;
+        if (base < need && need <= base + own) {
+          for (int i = 0; i <= pl.last; ++i) {
+            const bool here = i < rounds && key_of(__ldg(x + pl.at(i))) == from;
+            const uint32_t on = __ballot_sync(0xffffffffu, here);
+            if (here && base + __popc(on & ((1u << lane) - 1u)) + 1 == need)
+              for (int r = 0; r < C; ++r)
+                peer_store64(&s.threshold, r, entry_of(from, (uint32_t)pl.at(i)));
+            base += __popc(on);
+          }
+        }
+        row_sync<C>();
+        threshold = s.threshold;
+      }
     }
-    __syncthreads();
-    if (sh_total) {  // fewer than K selectable scores: take them all
-      all = true;
-      break;
+    if (inside <= kList) {
+      // The listed ones of the warp's positions.
+      const int first = pl.begin + (tid >> 5) * pl.seg, end = min(first + pl.seg, pl.begin + pl.len);
+      for (int i = lane; i < (int)inside; i += 32) {
+        const uint64_t e = s.mine[i];
+        const int p = (int)~(uint32_t)e;
+        count += e >= threshold && p >= first && p < end ? 1u : 0u;
+      }
     }
-    prefix = sh_prefix;
-    need = sh_need;
-    __syncthreads();
   }
-  int done = 0, ties = 0;
-  for (int64_t i0 = 0; i0 < n; i0 += kLongThreads) {
-    const int64_t i = i0 + tid;
-    const uint32_t k = i < n ? key_of(x[i]) : 0u;
-    const bool gt = all ? k > kNegInf : k > prefix;
-    const bool eq = !all && i < n && k == prefix;
-    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) {
-      warp_gt[warp] = __popc(mg);
-      warp_eq[warp] = __popc(me);
+
+  uint32_t base = count_before<T, C>(s, rank, count);
+  for (int i = 0; i <= pl.last; i += 8) {
+    float v[8];
+    load(i, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool here = entry_of(key_of(v[j]), (uint32_t)pl.at(i + j)) >= threshold;
+      const uint32_t on = __ballot_sync(0xffffffffu, here);
+      if (here) o[base + __popc(on & ((1u << lane) - 1u))] = pl.at(i + j);
+      base += __popc(on);
     }
-    __syncthreads();
-    const int vg = warp_gt[lane], ve = warp_eq[lane];
-    const uint32_t below = (1u << lane) - 1u;
-    const int g = done + __reduce_add_sync(0xffffffffu, lane < warp ? vg : 0) + __popc(mg & below);
-    const int e = ties + __reduce_add_sync(0xffffffffu, lane < warp ? ve : 0) + __popc(me & below);
-    // Position in the output: those above before it plus the ties taken.
-    const int at = g + min(e, (int)need);
-    if (gt) o[all ? g : at] = (int32_t)i;
-    if (eq && e < (int)need) o[at] = (int32_t)i;
-    done += __reduce_add_sync(0xffffffffu, vg);
-    ties += __reduce_add_sync(0xffffffffu, ve);
-    __syncthreads();
   }
-  const int filled = all ? done : K;
-  for (int i = filled + tid; i < K; i += kLongThreads) o[i] = -1;
+  for (uint32_t i = min(row_able, (uint32_t)K) + rank * T + tid; i < (uint32_t)K; i += C * T) o[i] = -1;
+  row_sync<C>();  // no block leaves while another reads its shared memory
 }
 
 }  // namespace
@@ -805,9 +905,10 @@ extern "C" int sas_topk_select(const float* scores, int64_t score_stride, const 
   else if (num_keys <= 32 * 1024) SAS_TOPK(1024, 1, 32);
   else if (num_keys <= 32 * 1024 * 2) SAS_TOPK(1024, 2, 32);
   else if (num_keys <= 32 * 1024 * 4) SAS_TOPK(1024, 4, 32);
+  else if (num_keys <= 32 * 1024 * 8) SAS_TOPK(1024, 8, 32);
   else
-    topk_long_kernel<<<rows, kLongThreads, 0, stream>>>(scores, score_stride, lengths, num_keys,
-                                                        topk, indices);
+    topk_long_kernel<<<(unsigned)rows * kLongBlocks, kLongThreads, 0, stream>>>(
+        scores, score_stride, lengths, num_keys, topk, indices);
 #undef SAS_TOPK
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }

@@ -484,6 +484,20 @@ def test_gpu_select_topk_many_rows(rows, N, K, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows, N, K", [(3, 200001, 2048), (3, 270001, 700), (2, 600011, 5000),
+                                        (1, 1000003, 300000)])
+def test_gpu_select_topk_long_rows(rows, N, K, kind):
+    g = torch.Generator().manual_seed(N + K)
+    x = topk_rows(kind, rows, N, g)
+    lengths = torch.randint(0, N + 1, (rows,), generator=g, dtype=torch.int32)
+    d = x.cuda()
+    assert np.array_equal(indexer.select_topk(d, K)[:, 0].cpu().numpy(), topk_reference(x, K))
+    got = indexer.select_topk(d, K, lengths=lengths.cuda())
+    assert np.array_equal(got[:, 0].cpu().numpy(), topk_reference(x, K, lengths))
+
+
+@pytest.mark.gpu
 def test_gpu_select_topk_strides_lengths_and_stream():
     g = torch.Generator().manual_seed(3)
     x = torch.randn(6, 1003, generator=g)
