@@ -188,6 +188,7 @@ def lib() -> C.CDLL:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 class on_device:
@@ -202,7 +203,7 @@ class on_device:
         self.guard = None
 
     def __enter__(self) -> int:
-        if torch.cuda.current_device() != self.dev.index:
+        if _get_device() != self.dev.index:
             self.guard = torch.cuda.device(self.dev)
             self.guard.__enter__()
         if _raw_stream is not None:

@@ -386,7 +386,8 @@ def test_gpu_refusals():
 
 
 @pytest.mark.gpu
-def test_gpu_sizes_at_their_ends():
+def test_gpu_sizes_at_their_ends(monkeypatch):
+    monkeypatch.delenv("SAS_CHECK_DEVICE_ERRORS", raising=False)
     case = score_case(13, (2,), (50,), 4, 64, 16)
     q, w, pool, table, cu, kv, _, N = case
     good = dict(q=q.cuda(), weights=w.cuda(), key_pool=pool.cuda(), block_table=table.cuda(),
@@ -406,6 +407,10 @@ def test_gpu_sizes_at_their_ends():
         s, n = indexer.index_scores(max_keys=9, return_lengths=True, **{**good, **change})
         assert bool((s == NEG).all()) and s.shape == (2, 9) and n.tolist() == [9, 9]
         assert bool((indexer.select_keys(topk=3, max_keys=9, **{**good, **change}) == -1).all())
+    # A page of an empty pool is one past it: reported, where that is asked for.
+    monkeypatch.setenv("SAS_CHECK_DEVICE_ERRORS", "1")
+    with pytest.raises(RuntimeError, match="site=53"):
+        indexer.index_scores(**{**good, "key_pool": pool.cuda()[:0]})
 
 
 # ---- on a GPU: selection ----
