@@ -148,19 +148,20 @@ struct Turn {
   float4 cs[2], sn[2];
 };
 
+template <bool kInter>
 __device__ __forceinline__ Turn load_turn(const RowArgs& a, const uint16_t* src, int64_t pos,
                                           int i) {
   const int rot0 = a.dim - 2 * a.half;
   Turn t;
-  t.c = 8 * i < (a.interleaved ? 2 * a.half : a.half) ? rot0 + 8 * i : -1;
+  t.c = 8 * i < (kInter ? 2 * a.half : a.half) ? rot0 + 8 * i : -1;
   if (t.c >= 0) {
-    const size_t o = (size_t)pos * a.half + (a.interleaved ? 4 * i : 8 * i);
+    const size_t o = (size_t)pos * a.half + (kInter ? 4 * i : 8 * i);
     const float4* cp = reinterpret_cast<const float4*>(a.cosv + o);
     const float4* sp = reinterpret_cast<const float4*>(a.sinv + o);
     t.x = *reinterpret_cast<const uint4*>(src + t.c);
     t.cs[0] = __ldg(cp);
     t.sn[0] = __ldg(sp);
-    if (!a.interleaved) {
+    if (!kInter) {
       t.y = *reinterpret_cast<const uint4*>(src + t.c + a.half);
       t.cs[1] = __ldg(cp + 1);
       t.sn[1] = __ldg(sp + 1);
@@ -169,12 +170,12 @@ __device__ __forceinline__ Turn load_turn(const RowArgs& a, const uint16_t* src,
   return t;
 }
 
-template <bool kBf16, Weights kW>
+template <bool kBf16, Weights kW, bool kInter>
 __device__ __forceinline__ void store_turn(const RowArgs& a, const Turn& t, uint16_t* dst,
                                            float scale, const float* sw) {
   if (t.c < 0) return;
   Eight e = norm8<kBf16, kW>(a, t.x, scale, t.c, sw);
-  if (a.interleaved) {
+  if constexpr (kInter) {
     const float co[4] = {t.cs[0].x, t.cs[0].y, t.cs[0].z, t.cs[0].w};
     const float si[4] = {t.sn[0].x, t.sn[0].y, t.sn[0].z, t.sn[0].w};
 #pragma unroll
@@ -219,14 +220,14 @@ __device__ __forceinline__ void load_row(const RowArgs& a, const uint16_t* src, 
 // rotation position, checked by the caller.  src == dst is allowed: what a
 // lane stores, no other lane reads, but for the norm's pass, which the lanes'
 // reduction ends.
-template <int V, bool kBf16, Weights kW>
+template <int V, bool kBf16, Weights kW, bool kInter>
 __device__ __forceinline__ void transform_row(const RowArgs& a, uint4 (&raw)[V],
                                               const uint16_t* src, uint16_t* dst, int64_t pos,
                                               int gl, uint32_t mask, const float* sw) {
   const int straight = a.dim - 2 * a.half;  // columns before the rotated ones
   Turn t;
   t.c = -1;
-  if (a.half > 0) t = load_turn(a, src, pos, gl);
+  if (a.half > 0) t = load_turn<kInter>(a, src, pos, gl);
   float scale = 1.0f;
   if (a.norm_dim > 0) {
     uint64_t sum2 = 0;
@@ -256,9 +257,9 @@ __device__ __forceinline__ void transform_row(const RowArgs& a, uint4 (&raw)[V],
       *reinterpret_cast<uint4*>(dst + c) =
           pack8<kBf16>(norm8<kBf16, kW>(a, raw[v], scale, c, sw));
   }
-  store_turn<kBf16, kW>(a, t, dst, scale, sw);
+  store_turn<kBf16, kW, kInter>(a, t, dst, scale, sw);
   for (int i = gl + kLanes; 4 * i < a.half; i += kLanes)
-    store_turn<kBf16, kW>(a, load_turn(a, src, pos, i), dst, scale, sw);
+    store_turn<kBf16, kW, kInter>(a, load_turn<kInter>(a, src, pos, i), dst, scale, sw);
 }
 
 __device__ __forceinline__ void note_error(int32_t* err, int site, int detail, int extra) {
@@ -285,13 +286,21 @@ struct HeadArgs {
   bool pos64;
 };
 
-// Persistent where there are more rows than the blocks that fit: two blocks an
-// SM, 16 warps with 4 rows each in flight (74 KB of 576 columns), weights in
-// shared memory.  On 8192 x 128 rows of 576 columns this takes 383 us (6.3 TB/s,
+// Blocks an SM: two, or where rows of up to 256 columns leave room, as many as
+// fit without spills.  8192 x 64 rows of 128 columns, all normed and 64 rotated,
+// take 61 us with four, 96 us with two, 67 us with five (spills); by halves, which
+// hold both columns' vectors, 81 us with three, 102 us with two, 87 us with four.
+__host__ __device__ constexpr int blocks_per_sm(int v, bool interleaved) {
+  return v > 4 ? 2 : interleaved ? 4 : 3;
+}
+
+// Persistent where there are more rows than the blocks that fit: of 576 columns
+// 16 warps an SM with 4 rows each in flight (74 KB), weights in shared memory.  On 8192 x 128 rows of 576 columns this takes 383 us (6.3 TB/s,
 // 96 % of the measured copy rate); a block for every 32 rows 467 us, with the
 // weights read from global memory a row.
-template <int V, bool kBf16, Weights kW>
-__global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(RowArgs a, HeadArgs h) {
+template <int V, bool kBf16, Weights kW, bool kInter>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(V, kInter))
+    norm_rope_kernel(RowArgs a, HeadArgs h) {
   __shared__ alignas(16) float sw[kW == kShared ? SAS_MAX_ROW_DIM : 4];
   if constexpr (kW == kShared) {
     for (int c = threadIdx.x * 8; c < a.norm_dim; c += kThreads * 8) {
@@ -321,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(RowArgs a, HeadA
         continue;
       }
     }
-    transform_row<V, kBf16, kW>(a, raw, src, dst, pos, gl, row_mask(), sw);
+    transform_row<V, kBf16, kW, kInter>(a, raw, src, dst, pos, gl, row_mask(), sw);
   }
 }
 
@@ -339,7 +348,7 @@ struct AppendArgs {
 // probes, the page, the row): the row itself is asked for first.  8 x 4096 rows
 // of 576 columns take 25 us, twice what their bytes need: 3.5 rounds of such
 // chains.
-template <int V, bool kBf16, Weights kW>
+template <int V, bool kBf16, Weights kW, bool kInter>
 __global__ void __launch_bounds__(kThreads, 2)
     append_norm_rope_kernel(RowArgs a, AppendArgs p) {
   const int64_t row64 = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
@@ -382,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (gl == 0) note_error(p.err, 51, row, lo);
     return;
   }
-  transform_row<V, kBf16, kW>(
+  transform_row<V, kBf16, kW, kInter>(
       a, raw, src,
       p.pool + ((size_t)blk * p.block_size + (size_t)(pos - lb * p.block_size)) * a.dim, rot, gl,
       mask, nullptr);
@@ -423,14 +432,13 @@ int row_args(const SasRowTransform* tr, RowArgs* a) {
   return SAS_OK;
 }
 
-// Calls LAUNCH(V, bf16, weights) with the vectors a lane that hold a row; kind:
-// where weights are read, if any.
+// Calls LAUNCH(V, bf16, weights) with the vectors a lane that hold a row.
 #define SAS_ROW_TYPES(V, LAUNCH)                                          \
   do {                                                                    \
     const bool weighted = a.weight != nullptr && a.norm_dim > 0;          \
-    if (bf16 && weighted) LAUNCH(V, true, kind);                          \
+    if (bf16 && weighted) LAUNCH(V, true, kGlobal);                          \
     else if (bf16) LAUNCH(V, true, kNone);                                \
-    else if (weighted) LAUNCH(V, false, kind);                            \
+    else if (weighted) LAUNCH(V, false, kGlobal);                            \
     else LAUNCH(V, false, kNone);                                         \
   } while (0)
 #define SAS_ROW_DISPATCH(LAUNCH)                                          \
@@ -473,17 +481,23 @@ extern "C" int sas_norm_rope(const SasRowTransform* tr, const void* x, int64_t x
   int dev = 0;
   const int sms = sas::current_device_sms(&dev);
   if (sms <= 0) return SAS_ERR_CUDA;
-  const unsigned blocks = blocks_of(rows), full = 2u * (unsigned)sms;
-#define SAS_HEADS(V, B, W) norm_rope_kernel<V, B, W><<<grid, kThreads, 0, stream>>>(a, h)
-  if (blocks > full) {
-    constexpr Weights kind = kShared;
-    const unsigned grid = full;
-    SAS_ROW_DISPATCH(SAS_HEADS);
-  } else {
-    constexpr Weights kind = kGlobal;
-    const unsigned grid = blocks;
-    SAS_ROW_DISPATCH(SAS_HEADS);
-  }
+  const unsigned blocks = blocks_of(rows);
+#define SAS_HEADS_OF(V, B, W, I)                                                      \
+  do {                                                                                \
+    const unsigned full = (unsigned)(blocks_per_sm(V, I) * sms);                      \
+    if (blocks > full)                                                                \
+      norm_rope_kernel<V, B, (W) == kGlobal ? kShared : (W), I>                       \
+          <<<full, kThreads, 0, stream>>>(a, h);                                      \
+    else                                                                              \
+      norm_rope_kernel<V, B, W, I><<<blocks, kThreads, 0, stream>>>(a, h);            \
+  } while (0)
+#define SAS_HEADS(V, B, W)                       \
+  do {                                           \
+    if (a.interleaved) SAS_HEADS_OF(V, B, W, true); \
+    else SAS_HEADS_OF(V, B, W, false);           \
+  } while (0)
+  SAS_ROW_DISPATCH(SAS_HEADS);
+#undef SAS_HEADS_OF
 #undef SAS_HEADS
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;
 }
@@ -508,9 +522,13 @@ extern "C" int sas_kv_append_norm_rope(const SasRowTransform* tr, void* pool, in
                      total_new, cmp_ratio};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const bool bf16 = tr->dtype == SAS_DTYPE_BF16;
-  constexpr Weights kind = kGlobal;
-#define SAS_APPEND(V, B, W) \
-  append_norm_rope_kernel<V, B, W><<<blocks_of(total_new), kThreads, 0, stream>>>(a, p)
+#define SAS_APPEND(V, B, W)                                                                     \
+  do {                                                                                          \
+    if (a.interleaved)                                                                          \
+      append_norm_rope_kernel<V, B, W, true><<<blocks_of(total_new), kThreads, 0, stream>>>(a, p); \
+    else                                                                                        \
+      append_norm_rope_kernel<V, B, W, false><<<blocks_of(total_new), kThreads, 0, stream>>>(a, p); \
+  } while (0)
   SAS_ROW_DISPATCH(SAS_APPEND);
 #undef SAS_APPEND
   return cudaGetLastError() == cudaSuccess ? SAS_OK : SAS_ERR_CUDA;

@@ -218,6 +218,25 @@ def test_gpu_norm_rope_many_rows_and_wide_rotations(D, rope, norm, wt, inter):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D, rope, norm, wt, inter", [
+    *[ROWS[i] for i in (6, 7, 8, 9, 10)], (128, 64, 128, "row", True), (256, 256, 128, None, True),
+    (256, 64, 256, torch.float32, False), (64, 64, 0, None, False)])
+def test_gpu_norm_rope_many_narrow_rows(D, rope, norm, wt, inter, dtype):
+    from sparse_attn_sharedkv_b200.rope import norm_rope
+    T, H = 641, 32
+    x, cos, sin, w, _ = row_case(D, rope, norm, wt, dtype, T * H, D + rope)
+    x = x.view(T, H, D)
+    pos = torch.randint(0, 4096, (T,), generator=torch.Generator().manual_seed(T)).cuda()
+    kw = dict(norm_dim=norm, norm_weight=w, eps=EPS, interleaved=inter)
+    want, mag = reference(x, pos[:, None].expand(T, H), cos, sin, norm, w, inter)
+    y = norm_rope(x, pos, cos, sin, **kw)
+    check(y, want, mag, dtype)
+    norm_rope(x, pos, cos, sin, out=x, **kw)
+    assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
 def test_gpu_norm_rope_strided_and_far_apart():
     from sparse_attn_sharedkv_b200.rope import norm_rope
     x, cos, sin, w, _ = row_case(576, 64, 512, torch.float32, torch.bfloat16, 5 * 7 * 2, 3)
