@@ -199,9 +199,9 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
 }
 
 // relu that keeps NaN.
-__device__ __forceinline__ float relu_nan(uint32_t bits) {
+__device__ __forceinline__ float relu_nan(float x) {
   float y;
-  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(__uint_as_float(bits)));
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -394,6 +394,12 @@ __device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_
   uint64_t w[kIxHalf / 2];
 #pragma unroll
   for (int i = 0; i < kIxHalf / 2; ++i) w[i] = 0;
+  // The least of a product and its column's limit: the product where the limit
+  // is NaN, 0 or less (also for NaN) where it is 0, in the piece of 16 columns in
+  // which the heads end.
+  float limit[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) limit[k] = k < p.num_heads % 16 ? CUDART_NAN_F : 0.0f;
   int n = 0, u = 0, m = 0;  // tiles of the pair, of this half, items with tiles
   for (int i = 0; i < count; ++i) {
     const IxInfo* info = ix_next(ctl, i, p.err, 73);
@@ -447,26 +453,34 @@ __device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_
             if (lane == 0) arrive_remote(empty0 + 8u * (uint32_t)b);
           }
           // Columns of padded heads stay out of the sum: their products are zero,
-          // but NaN with a key of infinities. (Without the template argument the
-          // branches cost heads that fill the tile 20 %: 1046 -> 1240 us for
-          // 8 x 4096 tokens of 64 heads.)
-          const int heads = kPadded ? p.num_heads - 16 * c % kHp : 16;  // of this piece
-          if (heads >= 16) {
+          // but NaN with a key of infinities.  They are in the upper half of a
+          // token's columns, for which alone there are branches.  (Without the
+          // template argument they cost heads that fill the tile 20 %: 1046 ->
+          // 1240 us for 8 x 4096 tokens of 64 heads.  4096 tokens of 48 heads take 138
+          // us, 149 with branches in both halves and a select for each column, and
+          // 134 with 64 heads; 24 heads 110, 115 and, with 32, 87 us.)
+          const bool upper = kPadded && 16 * (c % kPieces) + 16 > kHp / 2;
+          const int heads = upper ? p.num_heads - 16 * (c % kPieces) : 16;  // of this piece
+          if (heads > 0) {
+            const bool ends = upper && heads < 16;
+            auto add = [&](bool cut) {
 #pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-              const uint32_t* x = &v[c & 1][k];
-              s0 = fma2(w[8 * c + k / 2], pack_f32(relu_nan(x[0]), relu_nan(x[1])), s0);
-              s1 = fma2(w[8 * c + k / 2 + 1], pack_f32(relu_nan(x[2]), relu_nan(x[3])), s1);
-            }
-          } else if (heads > 0) {
+              for (int k = 0; k < 16; k += 4) {
+                float x[4];
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-              const uint32_t* x = &v[c & 1][k];
-              s0 = fma2(w[8 * c + k / 2],
-                        pack_f32(k < heads ? relu_nan(x[0]) : 0.0f,
-                                 k + 1 < heads ? relu_nan(x[1]) : 0.0f),
-                        s0);
-            }
+                for (int j = 0; j < 4; ++j) {
+                  x[j] = __uint_as_float(v[c & 1][k + j]);
+                  if (cut) x[j] = fminf(x[j], limit[k + j]);
+                  x[j] = relu_nan(x[j]);
+                }
+                s0 = fma2(w[8 * c + k / 2], pack_f32(x[0], x[1]), s0);
+                s1 = fma2(w[8 * c + k / 2 + 1], pack_f32(x[2], x[3]), s1);
+              }
+            };
+            if (ends)
+              add(true);
+            else
+              add(false);
           }
           if ((c + 1) % kPieces == 0) {
             if (key < len[tok] || (p.fill && key < p.num_keys))

@@ -257,6 +257,20 @@ def test_gpu_index_scores_infinite_key(H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H", [1, 12, 16, 20, 33, 63, 64, 100, 127])
+def test_gpu_index_scores_nan_in_the_last_head(H):
+    g = torch.Generator().manual_seed(H)
+    q = torch.randn(2, H, 64, generator=g).to(torch.bfloat16)
+    w = torch.randn(2, H, generator=g)
+    pool = torch.randn(4, 64, 1, 64, generator=g).to(torch.bfloat16)
+    case = (q, w, pool, torch.tensor([[2, 1, 0]], dtype=torch.int32), [0, 2], [150], 1, 150)
+    clean = run_scores(case)
+    q[0, H - 1, 5] = float("nan")
+    s = run_scores(case)
+    assert s[0, :149].isnan().all() and s[0, 149] == NEG and torch.equal(s[1], clean[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H, D, bs", [(16, 128, 64), (64, 128, 64), (128, 64, 48), (40, 128, 20)])
 def test_gpu_index_scores_long_runs(H, D, bs):
     # Rows of 131072 keys, so that each pair of CTAs goes through its buffers many times, and
