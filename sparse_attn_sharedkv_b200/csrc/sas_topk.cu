@@ -21,8 +21,8 @@
 //      winners are marked for the threads that hold them;
 //   5. the selected positions are counted and written.
 //
-// Any other row (infinities, NaN, a single value, more left than the lists
-// hold) is read again as unsigned keys of the same order: histograms linear
+// Scores of -inf are left out of all of this.  Any other row (+inf, NaN, a single
+// value, more left than the lists hold) is read again as unsigned keys of the same order: histograms linear
 // in the keys divide the range of the border keys by at least 512 a round
 // until 128 or a single key are left; equal keys are taken by a count over
 // their positions.
@@ -521,18 +521,40 @@ __global__ void __launch_bounds__(T, C == 1 ? 1024 / T : 1) __cluster_dims__(C, 
   }
 
   uint32_t sel = 0, able = (uint32_t)n;  // bit i of sel: v[i] is selected
-  const float scale = __fdividef((float)(kBins - 2), high - low);
+  uint32_t valid = rounds < 32 ? (1u << rounds) - 1u : 0xffffffffu;  // bits of scores that count
   bool general = true;
   if (short_row && low > -CUDART_INF_F) return;
-  if (!short_row && low > -CUDART_INF_F && high < CUDART_INF_F && scale > 0.0f &&
+  // Scores of -inf (there is no NaN then) do not count: the extremes again without
+  // them.  4096 rows of 16384, a third of them masked: 168 us, as keys 314 us,
+  // without a mask 135 us.
+  if (low == -CUDART_INF_F) {
+    uint32_t kmin = 0xffffffffu, kmax = 0;
+    able = 0;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if (i % kStep == 0 && i > last) break;
+      const bool on = i < rounds && v[i] > -CUDART_INF_F;
+      sel |= (on ? 1u : 0u) << i;
+      kmin = min(kmin, on ? key_of(v[i]) : 0xffffffffu);
+    }
+    valid = sel;
+    able = __popc(sel);
+    row_sync<C>();  // the extremes have been read
+    row_reduce<T, C>(s, rank, kmin, kmax, able);
+    low = score_of(kmin);
+    general = able > (uint32_t)K;
+  }
+  const float scale = __fdividef((float)(kBins - 2), high - low);
+  if (general && low > -CUDART_INF_F && high < CUDART_INF_F && scale > 0.0f &&
       scale < CUDART_INF_F) {
+    sel = 0;
     uint32_t need = (uint32_t)K;
     // 2^23 plus the bin of a score, rounded: non-decreasing in the score.
     auto place = [&](float a) { return fmaf(a - low, scale, kShift); };
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       if (i % kStep == 0 && i > last) break;
-      if (i < rounds)
+      if (valid >> i & 1)
         atomicAdd(&s.hist[kShiftBits + (kBins - 1) - __float_as_uint(place(v[i]))], 1u);
     }
     find_bin<T, C>(s, need);
@@ -575,8 +597,7 @@ __global__ void __launch_bounds__(T, C == 1 ? 1024 / T : 1) __cluster_dims__(C, 
         cand |= (t == bin ? 1u : 0u) << i;
         if (t == bin) border = v[i];
       }
-      const uint32_t valid = rounds < 32 ? (1u << rounds) - 1u : 0xffffffffu;
-      const int kept = cand > valid ? -1 : 31 - __clz(cand);  // the bit `border` belongs to
+      const int kept = (cand & ~valid) != 0 ? -1 : 31 - __clz(cand);  // the bit `border` belongs to
       sel &= valid;
       cand &= valid;
       auto score_at = [&](int i) { return i == kept ? border : __ldg(x + pl.at(i)); };
