@@ -112,6 +112,18 @@ __device__ __forceinline__ void row_sync() {
             : "memory");
 }
 
+// A block's shared memory may be written by its peers once it runs: every block of
+// a cluster arrives when it starts and waits before it first reaches for another's,
+// the loads of the scores in between.
+template <int C>
+__device__ __forceinline__ void peers_arrive() {
+  if constexpr (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+template <int C>
+__device__ __forceinline__ void peers_wait() {
+  if constexpr (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Shared memory of a block.
 template <int T, int C>
 struct TopkShared {
@@ -461,6 +473,7 @@ __global__ void __launch_bounds__(T, C == 1 ? 1024 / T : 1) __cluster_dims__(C, 
     for (int i = rank * T + tid; i < K; i += C * T) o[i] = -1;
     return;
   }
+  peers_arrive<C>();
   const int part = (n + C - 1) / C;  // of the block
   const int begin = min(n, rank * part), end = min(n, begin + part);
   const Places pl(begin, end, T);
@@ -511,6 +524,7 @@ __global__ void __launch_bounds__(T, C == 1 ? 1024 / T : 1) __cluster_dims__(C, 
   low = warp_min(__uint_as_float(s.wmin[lane % W]));
   high = warp_max(__uint_as_float(s.wmax[lane % W]));
   if constexpr (C > 1) {
+    peers_wait<C>();
     if (warp == 0 && lane < C) {
       peer_store(&s.rmin[rank], lane, __float_as_uint(low));
       peer_store(&s.rmax[rank], lane, __float_as_uint(high));
@@ -748,6 +762,7 @@ __global__ void __launch_bounds__(kLongThreads, 1) __cluster_dims__(kLongBlocks,
     for (int i = rank * T + tid; i < K; i += C * T) o[i] = -1;
     return;
   }
+  peers_arrive<C>();
   const int part = (int)(((int64_t)n + C - 1) / C);
   const int begin = (int)min((int64_t)n, (int64_t)rank * part);
   const Places pl(begin, min(n - begin, part) + begin, T);
@@ -778,6 +793,7 @@ __global__ void __launch_bounds__(kLongThreads, 1) __cluster_dims__(kLongBlocks,
     }
   });
   uint32_t row_able = able;
+  peers_wait<C>();
   row_reduce<T, C>(s, rank, kmin, kmax, row_able);
 
   uint64_t threshold = (uint64_t)(kNegInf + 1) << 32;  // entries from it on are selected
