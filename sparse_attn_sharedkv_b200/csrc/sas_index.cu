@@ -147,7 +147,8 @@ __device__ __forceinline__ int ix_local(const SasIndexParams& p, int b) {
 // span.  (Groups first, an even number of spans gave half of the pairs all the
 // late spans, which causal tokens mostly do not see: 4096 of them with 64 heads
 // took 230 us against 146.)  The tokens behind the
-// last sequence are those of a sequence p.batch that sees no key.
+// last sequence are those of a sequence p.batch that sees no key; those before the
+// first are in no group (ix_items fills their rows).
 __device__ __forceinline__ IxInfo ix_item(const IxArgs& a, int item, int lane, int* t1) {
   const SasIndexParams& p = a.p;
   const int tq = 1 << a.tq_shift;
@@ -494,7 +495,7 @@ __device__ __forceinline__ void ix_epilogue(const IxArgs& a, IxCtl& ctl, uint32_
   }
 }
 
-// Items, their queries and weights, and the fill.
+// Items, their queries and weights, and the fills.
 template <int kChunks, int kHp>
 __device__ __forceinline__ void ix_items(const IxArgs& a, IxCtl& ctl, uint32_t sQ, int count,
                                          int pair, int pairs, const CUtensorMap* tm_q, int rank,
@@ -576,6 +577,14 @@ __device__ __forceinline__ void ix_items(const IxArgs& a, IxCtl& ctl, uint32_t s
         }
       }
     }
+  }
+  // The tokens before the first sequence, of which no group has any, see no key.
+  const int lost = ix_local(p, 0);
+  for (int t = 2 * pair + rank; t < lost; t += 2 * pairs) {
+    if (p.lengths != nullptr && lane == 0) p.lengths[t] = 0;
+    if (p.fill)
+      for (int c = lane; c < p.num_keys; c += 32)
+        p.scores[(size_t)t * p.score_stride + c] = -CUDART_INF_F;
   }
   // The leader's barriers count the queries of both CTAs.
   if (rank == 0)

@@ -117,9 +117,10 @@ def index_scores(q: torch.Tensor, weights: torch.Tensor, *, key_pool: torch.Tens
                  ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Index scores of each token against the keys of its sequence.
 
-    q:            [T, H, D] (TND, with cu_seqlens_q [B + 1], prefix sums from 0) or
-                  [B, S, H, D] (BSND; tokens past a given q_len see no key), bf16 / fp16,
-                  H in 1..128, D a multiple of 8 up to 128.
+    q:            [T, H, D] (TND, with cu_seqlens_q [B + 1]: tokens before its first and at
+                  or past its last entry see no key) or [B, S, H, D] (BSND; tokens past a
+                  given q_len see no key), bf16 / fp16, H in 1..128, D a multiple of 8 up to
+                  128.
     weights:      float32 [T, H] / [B, S, H]; any softmax or width scale is folded in.
     key_pool:     [blocks, block_size, 1, D] index keys, q's dtype; block_table
                   [B, table_len] int32.  A position whose page is -1 or past the table

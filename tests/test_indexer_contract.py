@@ -1,0 +1,71 @@
+"""What ``include/sas.h`` says of ``sas_index_scores`` beyond the scores themselves."""
+
+import numpy as np
+import pytest
+import torch
+
+from sparse_attn_sharedkv_b200 import _lib, indexer
+
+from .test_indexer import NEG, check_scores, score_case, scores_reference, thresholds, \
+    topk_reference
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32).cuda()
+
+
+def raw_scores(q, w, pool, table, cu, kv, cols, stride=None, scores=None, lengths=None, **change):
+    """``sas_index_scores`` of CUDA tensors, its outputs where the caller has them."""
+    T, H, D = q.shape
+    p = _lib.SasIndexParams(
+        q=q.data_ptr(), weights=w.data_ptr(), key_pool=pool.data_ptr(),
+        block_table=table.data_ptr(), cu_seqlens_q=cu.data_ptr(), kv_len=kv.data_ptr(),
+        scores=scores.data_ptr(), lengths=lengths.data_ptr() if lengths is not None else None,
+        batch=kv.numel(), total_tokens=T, num_heads=H, head_dim=D,
+        dtype=_lib.DTYPE_BF16 if q.dtype == torch.bfloat16 else _lib.DTYPE_FP16,
+        block_size=pool.shape[1], num_blocks=pool.shape[0], table_len=table.shape[1],
+        cmp_ratio=1, num_keys=cols, num_tokens=T, fill=1, score_stride=stride or cols)
+    for name, value in change.items():
+        setattr(p, name, value)
+    _lib.check("sas_index_scores", _lib.lib().sas_index_scores(
+        p, torch.cuda.current_stream().cuda_stream))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [8, 64, 128])
+@pytest.mark.parametrize("before, behind", [(1, 0), (3, 2), (17, 1), (400, 0)])
+def test_gpu_tokens_of_no_sequence(H, before, behind):
+    q_lens, kv = (5, 0, 9), (700, 30, 90)
+    q, w, pool, table, cu, _, _, N = score_case(31, q_lens, kv, H, 64, 16)
+    want, mag = scores_reference(q, w, pool, table, thresholds(cu, kv, 1), N)
+    lens = [0] * before + [n for _, n in thresholds(cu, kv, 1)] + [0] * behind
+    pad = lambda t: torch.cat([t[:1].expand(before, *t.shape[1:]), t,
+                               t[:1].expand(behind, *t.shape[1:])]).contiguous().cuda()
+    qp, wp, cup = pad(q), pad(w), i32([before + c for c in cu])
+    T = qp.shape[0]
+    # Outputs that held something else, so that a row left out shows.
+    scores = torch.full((T, N), 123.0, device="cuda")
+    lengths = torch.full((T,), 77, dtype=torch.int32, device="cuda")
+    raw_scores(qp, wp, pool.cuda(), table.cuda(), cup, i32(kv), N, scores=scores, lengths=lengths)
+    assert lengths.tolist() == lens
+    inside = scores[before:T - behind]
+    check_scores(inside, want, mag, H, 64)
+    assert bool((scores[:before] == NEG).all()) and bool((scores[T - behind:] == NEG).all())
+    # Without the fill their rows stay as they were.
+    left = torch.full((T, N), 123.0, device="cuda")
+    raw_scores(qp, wp, pool.cuda(), table.cuda(), cup, i32(kv), N, scores=left, lengths=lengths,
+               fill=0)
+    assert lengths.tolist() == lens and bool((left[:before] == 123.0).all())
+    assert bool((left[T - behind:] == 123.0).all())
+    # A part of the tokens that starts between the ones of no sequence.
+    first = before // 2
+    part = torch.full((T - first, N), 123.0, device="cuda")
+    raw_scores(qp, wp, pool.cuda(), table.cuda(), cup, i32(kv), N, scores=part,
+               lengths=lengths[first:], first_token=first, num_tokens=T - first)
+    assert torch.equal(part, scores[first:]) and lengths.tolist() == lens
+    # The selection of such a batch.
+    idx = indexer.select_keys(qp, wp, key_pool=pool.cuda(), block_table=table.cuda(),
+                              cu_seqlens_q=cup, seqused_kv=i32(kv), topk=40, max_keys=N)
+    assert np.array_equal(idx[:, 0].cpu().numpy(),
+                          topk_reference(scores.cpu().numpy(), 40, lens))
+    assert bool((idx[:before] == -1).all())
