@@ -381,12 +381,15 @@ __device__ __forceinline__ uint64_t global_ns() {
   return t;
 }
 
-__device__ void record_error(int* err, int code, int site, int detail) {
+__device__ void record_error(int* err, int code, int site, int detail, int extra) {
   if (err != nullptr && atomicCAS(err, 0, code) == 0) {
     err[1] = site;
     err[2] = detail;
-    err[3] = (int)blockIdx.x;
+    err[3] = extra;
   }
+}
+__device__ void record_error(int* err, int code, int site, int detail) {
+  record_error(err, code, site, detail, (int)blockIdx.x);
 }
 
 // Bounded wait; on timeout records the error and raises the CTA abort flag.

@@ -284,9 +284,9 @@ struct IxPage {
   }
 };
 
-// Row in the pool, no_row without a page.
-__device__ __forceinline__ int ix_row(const IxArgs& a, int id, int off) {
-  if (id >= a.p.num_blocks) record_error(a.p.err, SAS_ERR_DEVICE, 53, id);
+// Row in the pool of a key of sequence `batch`, no_row without a page.
+__device__ __forceinline__ int ix_row(const IxArgs& a, int id, int off, int batch) {
+  if (id >= a.p.num_blocks) record_error(a.p.err, SAS_ERR_DEVICE, 53, id, batch);
   return id < 0 || id >= a.p.num_blocks ? a.no_row : id * a.p.block_size + off;
 }
 
@@ -309,8 +309,8 @@ __device__ __forceinline__ void ix_keys(const IxArgs& a, IxCtl& ctl, uint32_t sK
   for (int i = 0; i < count; ++i) {
     const IxInfo* info = ix_next(ctl, i, p.err, 69);
     if (info == nullptr) return;
-    const int t0 = info->t0, tc = info->tc, most = info->most;
-    const int32_t* table = p.block_table + (size_t)info->batch * p.table_len;
+    const int t0 = info->t0, tc = info->tc, most = info->most, batch = info->batch;
+    const int32_t* table = p.block_table + (size_t)batch * p.table_len;
     ix_done(ctl, i, lane);
     if (tc == t0) continue;
     int t = t0 + ((n ^ half) & 1);
@@ -338,7 +338,7 @@ __device__ __forceinline__ void ix_keys(const IxArgs& a, IxCtl& ctl, uint32_t sK
       if (!ix_wait(ctl, &ctl.k_empty[s], ph, p.err, 70)) return;
       int rows[4];
       if (!gather) {
-        rows[0] = ix_row(a, id[0], pg.off);
+        rows[0] = ix_row(a, id[0], pg.off, batch);
         const uint32_t mapped = __ballot_sync(0xffffffffu, rows[0] != a.no_row);
         if (lane < 16) ctl.bits[slot][lane] = (mapped >> my_box) & 1 ? 255 : 0;
       } else {
@@ -346,7 +346,7 @@ __device__ __forceinline__ void ix_keys(const IxArgs& a, IxCtl& ctl, uint32_t sK
         uint32_t four = 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          rows[r] = ix_row(a, id[r], q.off);
+          rows[r] = ix_row(a, id[r], q.off, batch);
           four |= (rows[r] != a.no_row ? 1u : 0u) << r;
           q.advance(p, 0, 1);
         }

@@ -69,3 +69,23 @@ def test_gpu_tokens_of_no_sequence(H, before, behind):
     assert np.array_equal(idx[:, 0].cpu().numpy(),
                           topk_reference(scores.cpu().numpy(), 40, lens))
     assert bool((idx[:before] == -1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs", [5, 64])
+@pytest.mark.parametrize("bad", [0, 2, 3])
+def test_gpu_page_past_the_pool_names_its_sequence(bs, bad, monkeypatch):
+    kv = (333, 7, 200, 900)
+    q, w, pool, table, cu, _, _, N = score_case(9, (4, 1, 2, 1), kv, 24, 64, bs)
+    page = pool.shape[0] + 5
+    table[bad, 1] = page
+    table[1, 1] = page + 1  # of a position that its sequence does not have
+    if bs == 5:
+        table[1, 1:3] = torch.tensor([1, page + 1])
+    monkeypatch.setenv("SAS_CHECK_DEVICE_ERRORS", "1")
+    kw = dict(key_pool=pool.cuda(), block_table=table.cuda(), cu_seqlens_q=i32(cu),
+              seqused_kv=i32(kv), max_keys=N)
+    with pytest.raises(RuntimeError, match=f"code=6 site=53 detail={page} {bad}$"):
+        indexer.index_scores(q.cuda(), w.cuda(), **kw)
+    with pytest.raises(RuntimeError, match=f"code=6 site=53 detail={page} {bad}$"):
+        indexer.select_keys(q.cuda(), w.cuda(), topk=8, **kw)
