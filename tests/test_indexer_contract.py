@@ -89,3 +89,23 @@ def test_gpu_page_past_the_pool_names_its_sequence(bs, bad, monkeypatch):
         indexer.index_scores(q.cuda(), w.cuda(), **kw)
     with pytest.raises(RuntimeError, match=f"code=6 site=53 detail={page} {bad}$"):
         indexer.select_keys(q.cuda(), w.cuda(), topk=8, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset, spare", [(1, 0), (0, 1), (3, 6), (0, 0), (0, 4)])
+@pytest.mark.parametrize("cols", [257, 1023, 2051])
+def test_gpu_scores_of_any_alignment(cols, offset, spare):
+    # Rows that start anywhere and follow at any stride, columns several tiles behind the last
+    # position that a token sees; what lies between and behind the rows stays.
+    q, w, pool, table, cu, kv, _, _ = score_case(33, (9, 1, 4), (40, 700, 4), 24, 64, 16)
+    want, mag = scores_reference(q, w, pool, table, thresholds(cu, kv, 1), cols)
+    T, stride = q.shape[0], cols + spare
+    buf = torch.full((offset + T * stride + 8,), 123.0, device="cuda")
+    args = (q.cuda(), w.cuda(), pool.cuda(), table.cuda(), i32(cu), i32(kv), cols)
+    raw_scores(*args, stride=stride, scores=buf[offset:])
+    rows = buf[offset:offset + T * stride].view(T, stride)
+    check_scores(rows[:, :cols], want, mag, 24, 64)
+    kw = dict(key_pool=args[2], block_table=args[3], cu_seqlens_q=args[4], seqused_kv=args[5])
+    assert torch.equal(rows[:, :cols], indexer.index_scores(*args[:2], max_keys=cols, **kw))
+    buf.as_strided((T, cols), (stride, 1), offset).fill_(123.0)
+    assert bool((buf == 123.0).all())
