@@ -102,14 +102,14 @@ __device__ __forceinline__ uint32_t peer_add(void* p, int rank, uint32_t v) {
   return old;
 }
 
+// Barriers of a cluster here are not `.aligned` ones: loops over a lane's own scores
+// or entries end right before them.
 template <int C>
 __device__ __forceinline__ void row_sync() {
   if constexpr (C == 1)
     __syncthreads();
   else
-    asm volatile(
-        "barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-            : "memory");
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // A block's shared memory may be written by its peers once it runs: every block of
@@ -117,11 +117,11 @@ __device__ __forceinline__ void row_sync() {
 // the loads of the scores in between.
 template <int C>
 __device__ __forceinline__ void peers_arrive() {
-  if constexpr (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if constexpr (C > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
 }
 template <int C>
 __device__ __forceinline__ void peers_wait() {
-  if constexpr (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if constexpr (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Shared memory of a block.

@@ -50,6 +50,13 @@ def test_cluster_kernels_wait_for_their_peers():
             assert "C == 1" in m.group(), (name, m.group())
 
 
+def test_cluster_barriers_take_diverged_warps():
+    # Loops whose length differs between the lanes of a warp end right before some of them.
+    with open(os.path.join(CSRC, "sas_topk.cu")) as f:
+        barriers = re.findall(r"barrier\.cluster\.[\w.]+", f.read())
+    assert len(barriers) == 4 and not any("aligned" in b for b in barriers)
+
+
 # ---- on a GPU ----
 
 @pytest.mark.gpu
