@@ -25,13 +25,14 @@
 // are filled with -inf without loads.
 //
 // Bounds.  With few tokens a sequence the keys are read once each from HBM: 256
-// tokens of 64 heads against 32768 keys of 128 dims take 355 us, 6.2 TB/s of
-// keys and scores.  With many tokens the products and the epilogue share the
-// SM's issue slots and the power limit: 8 x 4096 causal tokens of 64 heads take
-// 990 us on a cool device and 1120 us in a run of such calls, of which the
-// products alone need 680 us at the burst rate of bf16 and 840 us at the
-// sustained one; an MMA of a half takes 64 cycles alone and about 100 beside
-// the two fp32 operations a column of the epilogue.
+// tokens of 64 heads against 32768 keys of 128 dims take 350 us, 6.2 TB/s of
+// keys and scores.  With many tokens the products: 8 x 4096 causal tokens of 64
+// heads take 1120 us in a run of such calls (1090 to 1250 us from device to
+// device), of which the products alone need 680 us at the burst rate of bf16 and
+// 840 us at the sustained one.  An MMA of a half takes 64 cycles alone and about
+// 100 beside the epilogue, with no unit saturated (tensor 58 %, ALU 50 %, issue
+// slots 51 %): whether the tiles wait for the epilogue's TMEM reads or for its
+// arithmetic has not been told apart.
 //
 // Warp roles in each CTA (384 threads, one CTA per SM):
 //   0, 3   keys, every other tile each: page lookup, TMA into a ring of stages
@@ -74,7 +75,8 @@ constexpr int kIxKChunk = kIxKeys * 128;   // 64 dims of a CTA's key tile
 constexpr int kIxSmem = 232448;            // the per-block opt-in maximum
 
 // Registers of the loading and issuing warpgroup and of an epilogue one: 88 +
-// 2 x 208 = 3 x 168, the launch's share of 384 threads.
+// 2 x 208 = 3 x 168, the launch's share of 384 threads.  (Of the instances only that of
+// 128 heads, all of them there, spills: 20 bytes.)
 constexpr int kIxRegsLoad = 88, kIxRegsEpi = 208;
 
 // An item as its roles need it: tokens tok0 .. tok0 + live (relative to the
@@ -570,7 +572,8 @@ __device__ __forceinline__ void ix_items(const IxArgs& a, IxCtl& ctl, uint32_t s
       for (int t = 0; t < r.live; ++t) {
         float* o2 = p.scores + (size_t)(r.tok0 + t) * p.score_stride;
         if (vec) {
-          for (int c = c0 + 4 * first; c + 4 <= c1; c += 256) *reinterpret_cast<float4*>(o2 + c) = none;
+          for (int c = c0 + 4 * first; c + 4 <= c1; c += 256)
+            *reinterpret_cast<float4*>(o2 + c) = none;
           if (first < (c1 & 3)) o2[(c1 & ~3) + first] = -CUDART_INF_F;
         } else {
           for (int c = c0 + first; c < c1; c += 64) o2[c] = -CUDART_INF_F;

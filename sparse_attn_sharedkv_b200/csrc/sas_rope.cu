@@ -287,17 +287,21 @@ struct HeadArgs {
 };
 
 // Blocks an SM: two, or where rows of up to 256 columns leave room, as many as
-// fit without spills.  8192 x 64 rows of 128 columns, all normed and 64 rotated,
-// take 61 us with four, 96 us with two, 67 us with five (spills); by halves, which
-// hold both columns' vectors, 81 us with three, 102 us with two, 87 us with four.
+// were fastest.  8192 x 64 rows of 128 columns, all normed and 64 rotated, take 61
+// us with four, 96 us with two, 67 us with five; by halves, which hold both columns'
+// vectors, 81 us with three, 102 us with two, 87 us with four.  (The bytes need 41
+// us.  By halves these instances spill 4 to 16 bytes, and the ones that read the
+// weights from global memory, for few rows, 16 to 48.)
 __host__ __device__ constexpr int blocks_per_sm(int v, bool interleaved) {
   return v > 4 ? 2 : interleaved ? 4 : 3;
 }
 
 // Persistent where there are more rows than the blocks that fit: of 576 columns
-// 16 warps an SM with 4 rows each in flight (74 KB), weights in shared memory.  On 8192 x 128 rows of 576 columns this takes 383 us (6.3 TB/s,
-// 96 % of the measured copy rate); a block for every 32 rows 467 us, with the
-// weights read from global memory a row.
+// 16 warps an SM with 4 rows each in flight (74 KB), weights in shared memory.  On
+// 8192 x 128 rows of 576 columns this takes 382 us in a loop over the same rows (6.3
+// TB/s, 97 % of the measured copy rate) and 400 us where the rows change from call to
+// call; a block for every 32 rows 467 us, with the weights read from global memory a
+// row.
 template <int V, bool kBf16, Weights kW, bool kInter>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(V, kInter))
     norm_rope_kernel(RowArgs a, HeadArgs h) {
@@ -346,8 +350,9 @@ struct AppendArgs {
 
 // One row for each eight lanes.  Few rows are a chain of latencies (the search's
 // probes, the page, the row): the row itself is asked for first.  8 x 4096 rows
-// of 576 columns take 25 us, twice what their bytes need: 3.5 rounds of such
-// chains.
+// of 576 columns take 25 us (18 us with the rows in L2), twice what their bytes
+// need: this launch goes through 3.5 rounds of such chains, and every row reads
+// its weights from global memory.
 template <int V, bool kBf16, Weights kW, bool kInter>
 __global__ void __launch_bounds__(kThreads, 2)
     append_norm_rope_kernel(RowArgs a, AppendArgs p) {
@@ -436,9 +441,9 @@ int row_args(const SasRowTransform* tr, RowArgs* a) {
 #define SAS_ROW_TYPES(V, LAUNCH)                                          \
   do {                                                                    \
     const bool weighted = a.weight != nullptr && a.norm_dim > 0;          \
-    if (bf16 && weighted) LAUNCH(V, true, kGlobal);                          \
+    if (bf16 && weighted) LAUNCH(V, true, kGlobal);                       \
     else if (bf16) LAUNCH(V, true, kNone);                                \
-    else if (weighted) LAUNCH(V, false, kGlobal);                            \
+    else if (weighted) LAUNCH(V, false, kGlobal);                         \
     else LAUNCH(V, false, kNone);                                         \
   } while (0)
 #define SAS_ROW_DISPATCH(LAUNCH)                                          \
@@ -482,19 +487,19 @@ extern "C" int sas_norm_rope(const SasRowTransform* tr, const void* x, int64_t x
   const int sms = sas::current_device_sms(&dev);
   if (sms <= 0) return SAS_ERR_CUDA;
   const unsigned blocks = blocks_of(rows);
-#define SAS_HEADS_OF(V, B, W, I)                                                      \
-  do {                                                                                \
-    const unsigned full = (unsigned)(blocks_per_sm(V, I) * sms);                      \
-    if (blocks > full)                                                                \
-      norm_rope_kernel<V, B, (W) == kGlobal ? kShared : (W), I>                       \
-          <<<full, kThreads, 0, stream>>>(a, h);                                      \
-    else                                                                              \
-      norm_rope_kernel<V, B, W, I><<<blocks, kThreads, 0, stream>>>(a, h);            \
+#define SAS_HEADS_OF(V, B, W, I)                                           \
+  do {                                                                     \
+    const unsigned full = (unsigned)(blocks_per_sm(V, I) * sms);           \
+    if (blocks > full)                                                     \
+      norm_rope_kernel<V, B, (W) == kGlobal ? kShared : (W), I>            \
+          <<<full, kThreads, 0, stream>>>(a, h);                           \
+    else                                                                   \
+      norm_rope_kernel<V, B, W, I><<<blocks, kThreads, 0, stream>>>(a, h); \
   } while (0)
-#define SAS_HEADS(V, B, W)                       \
-  do {                                           \
+#define SAS_HEADS(V, B, W)                          \
+  do {                                              \
     if (a.interleaved) SAS_HEADS_OF(V, B, W, true); \
-    else SAS_HEADS_OF(V, B, W, false);           \
+    else SAS_HEADS_OF(V, B, W, false);              \
   } while (0)
   SAS_ROW_DISPATCH(SAS_HEADS);
 #undef SAS_HEADS_OF
@@ -522,12 +527,13 @@ extern "C" int sas_kv_append_norm_rope(const SasRowTransform* tr, void* pool, in
                      total_new, cmp_ratio};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const bool bf16 = tr->dtype == SAS_DTYPE_BF16;
-#define SAS_APPEND(V, B, W)                                                                     \
-  do {                                                                                          \
-    if (a.interleaved)                                                                          \
-      append_norm_rope_kernel<V, B, W, true><<<blocks_of(total_new), kThreads, 0, stream>>>(a, p); \
-    else                                                                                        \
-      append_norm_rope_kernel<V, B, W, false><<<blocks_of(total_new), kThreads, 0, stream>>>(a, p); \
+  const unsigned blocks = blocks_of(total_new);
+#define SAS_APPEND(V, B, W)                                                            \
+  do {                                                                                 \
+    if (a.interleaved)                                                                 \
+      append_norm_rope_kernel<V, B, W, true><<<blocks, kThreads, 0, stream>>>(a, p);   \
+    else                                                                               \
+      append_norm_rope_kernel<V, B, W, false><<<blocks, kThreads, 0, stream>>>(a, p);  \
   } while (0)
   SAS_ROW_DISPATCH(SAS_APPEND);
 #undef SAS_APPEND

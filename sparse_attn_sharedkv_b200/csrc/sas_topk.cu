@@ -22,10 +22,10 @@
 //   5. the selected positions are counted and written.
 //
 // Scores of -inf are left out of all of this.  Any other row (+inf, NaN, a single
-// value, more left than the lists hold) is read again as unsigned keys of the same order: histograms linear
-// in the keys divide the range of the border keys by at least 512 a round
-// until 128 or a single key are left; equal keys are taken by a count over
-// their positions.
+// value, more left than the lists hold) is read again as unsigned keys of the same
+// order: histograms linear in the keys divide the range of the border keys by at
+// least 512 a round until 128 or a single key are left; equal keys are taken by a
+// count over their positions.
 //
 // Each warp of a block holds neighbouring positions, 32 a round: loads are
 // coalesced for any row alignment, the count of the selected positions before
@@ -35,7 +35,7 @@
 // The floor is one read of the scores and one write of the positions; what
 // bounds many rows is the issue of instructions (70 % of the slots; about 60 a
 // score of a lane) with the latency of the phases.  32768 causal rows of up to
-// 4096, K 2048: 178 us (82 us of memory); 4000 rows of 16384 to 32768: 230 us; 64
+// 4096, K 2048: 172 us (82 us of memory); 4000 rows of 16384 to 32768: 230 us; 64
 // rows of 8192 to 32768: 12 us.
 
 #include <cuda_runtime.h>
@@ -450,8 +450,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // Rounds a thread: 32 make the barriers and scans of a row cheaper by half, 16
 // make its phases shorter (launcher).  1024 threads an SM, 64 registers each:
-// 30000 rows of 1500 to 2048, K 512, take 137 us so, 174 us with 2048 threads of
-// 32 registers, some of them spilled.
+// 30000 rows of 1500 to 2048, K 512, take 138 us so, 174 us with 2048 threads of
+// 32 registers, some of them spilled.  (Of the instances of one block a row, that of
+// 128 threads and 32 rounds spills 8 bytes; the way by keys, with 32 rounds, 52 to 96.)
 template <int T, int C, int P>
 __global__ void __launch_bounds__(T, C == 1 ? 1024 / T : 1) __cluster_dims__(C, 1, 1)
     topk_kernel(const float* __restrict__ scores, int64_t stride,
@@ -878,7 +879,8 @@ __global__ void __launch_bounds__(kLongThreads, 1) __cluster_dims__(kLongBlocks,
     }
     if (inside <= kList) {
       // The listed ones of the warp's positions.
-      const int first = pl.begin + (tid >> 5) * pl.seg, end = min(first + pl.seg, pl.begin + pl.len);
+      const int first = pl.begin + (tid >> 5) * pl.seg;
+      const int end = min(first + pl.seg, pl.begin + pl.len);
       for (int i = lane; i < (int)inside; i += 32) {
         const uint64_t e = s.mine[i];
         const int p = (int)~(uint32_t)e;
@@ -899,7 +901,8 @@ __global__ void __launch_bounds__(kLongThreads, 1) __cluster_dims__(kLongBlocks,
       base += __popc(on);
     }
   }
-  for (uint32_t i = min(row_able, (uint32_t)K) + rank * T + tid; i < (uint32_t)K; i += C * T) o[i] = -1;
+  const uint32_t filled = min(row_able, (uint32_t)K);
+  for (uint32_t i = filled + rank * T + tid; i < (uint32_t)K; i += C * T) o[i] = -1;
   row_sync<C>();  // no block leaves while another reads its shared memory
 }
 
@@ -919,12 +922,12 @@ extern "C" int sas_topk_select(const float* scores, int64_t score_stride, const 
   // the largest as it takes (a cluster's barriers and remote reads cost more
   // than a block's longer phases: 256 rows of 32768 take 23 us in blocks of 1024
   // threads and 63 us in clusters of four of 512) unless the rows are so few
-  // that the clusters fit the SMs side by side (16 rows 10.3 against 12.3 us).  Rows of up to 16384 take 32
-  // scores a thread where there are many of them: 4000 rows of 4096 to 8192 62 us
-  // (73 us with 16 a thread), 32768 of up to 4096 178 (197), but 8 rows of 4096
-  // 10.3 us (8.2); about 300 to 600 rows take the same time either way.
-#define SAS_TOPK(T, C, P)                                                                          \
-  topk_kernel<T, C, P><<<(unsigned)rows * C, T, 0, stream>>>(                                     \
+  // that the clusters fit the SMs side by side (16 rows 10.3 against 12.3 us).  Rows
+  // of up to 16384 take 32 scores a thread where there are many of them: 4000 rows of
+  // 4096 to 8192 62 us (73 us with 16 a thread), 32768 of up to 4096 178 (197), but 8
+  // rows of 4096 10.3 us (8.2); about 300 to 600 rows take the same time either way.
+#define SAS_TOPK(T, C, P)                                     \
+  topk_kernel<T, C, P><<<(unsigned)rows * C, T, 0, stream>>>( \
       scores, score_stride, lengths, rows, sms * (1024 / T), num_keys, topk, indices)
   int dev = 0;
   const int sms = sas::current_device_sms(&dev);

@@ -30,8 +30,9 @@ from . import _lib
 from .api import _check_device_errors, _dtype_code
 
 # Bytes of scores that select_keys holds at a time.  Fewer launches, and their tails,
-# gain more than scores that are still in L2: 8 x 4096 causal tokens take 1.13 ms so,
-# 1.37 ms with 64 MiB, 1.78 ms with 16 MiB and 1.11 ms with all 512 MiB.
+# gain more than scores that are still in L2: 8 x 4096 causal tokens take 1.27 ms so
+# (in the same run their scores 1.10 ms and the selection 0.17 ms), 1.32 ms with 64 MiB,
+# 1.59 ms with 16 MiB and 1.25 ms with all 512 MiB.
 _SCORE_WORKSPACE = 256 << 20
 
 

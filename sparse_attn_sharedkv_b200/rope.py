@@ -116,8 +116,9 @@ def norm_rope(x: torch.Tensor, positions: Optional[torch.Tensor] = None,
     norm_dim:    columns, from the first, that are normed together (0: no norm);
                  ``norm_weight`` [norm_dim] float32 or x's dtype, None for ones.
     inverse:     rotate by the negative angles.
-    out:         a tensor of x's shape and dtype to write; ``x`` itself works in place,
-                 any other overlap does not.
+    out:         a tensor of x's shape and dtype to write: the last dim contiguous, the
+                 others multiples of 8 elements, B and S one stride apart, 16-byte aligned.
+                 ``x`` itself works in place, any other overlap does not.
 
     Rows of a position outside the tables are zeros; with ``check_errors`` the call
     synchronises and raises RuntimeError for them.
